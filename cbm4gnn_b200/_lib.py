@@ -28,6 +28,9 @@ SOURCES = [
     os.path.join(_PKG_DIR, "csrc", "cbm_cluster.cu"),
     os.path.join(_PKG_DIR, "csrc", "cbm_lift.cpp"),
     os.path.join(_PKG_DIR, "csrc", "cbm_sequence.cpp"),
+    os.path.join(_PKG_DIR, "csrc", "cbm_classes.cu"),
+    os.path.join(_PKG_DIR, "csrc", "cbm_norm.cu"),
+    os.path.join(_PKG_DIR, "csrc", "cbm_update.cu"),
 ]
 HEADERS = [
     os.path.join(_ROOT, "include", "cbm_b200.h"),
@@ -38,6 +41,7 @@ HEADERS = [
     os.path.join(_PKG_DIR, "csrc", "cbm_launch.cuh"),
     os.path.join(_PKG_DIR, "csrc", "cbm_lift.h"),
     os.path.join(_PKG_DIR, "csrc", "cbm_map.cuh"),
+    os.path.join(_PKG_DIR, "csrc", "cbm_values.cuh"),
 ]
 _OBJ_DIR = os.path.join(_PKG_DIR, "build")
 
@@ -88,6 +92,15 @@ EXPORTED = [
     "cbm_b200_copy2d_async",
     "cbm_b200_spmm_update_static",
     "cbm_b200_selftest_wait",
+    "cbm_b200_class_log_probs",
+    "cbm_b200_class_log_probs_grad",
+    "cbm_b200_group_norm",
+    "cbm_b200_group_norm_grad",
+    "cbm_b200_group_norm_workspace",
+    "cbm_b200_orthogonalise",
+    "cbm_b200_orthogonalise_workspace",
+    "cbm_b200_orthogonal_step",
+    "cbm_b200_orthogonal_step_workspace",
 ]
 
 
@@ -225,6 +238,20 @@ def lib() -> ctypes.CDLL:
     sig("cbm_b200_spmm_update_static", c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int32,
         c_int32, c_void_p)
     sig("cbm_b200_selftest_wait", c_int32, c_int32, c_int32, c_void_p)
+    sig("cbm_b200_class_log_probs", c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int32, *[c_void_p] * 6)
+    sig("cbm_b200_class_log_probs_grad", c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int32,
+        *[c_void_p] * 7, c_int64, c_void_p)
+    sig("cbm_b200_group_norm_workspace", c_int64, c_int64, c_int64, c_int32, c_int32, c_int32)
+    sig("cbm_b200_group_norm", c_int32, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p,
+        c_void_p, c_int32, c_float, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p)
+    sig("cbm_b200_group_norm_grad", c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64,
+        c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p)
+    sig("cbm_b200_orthogonalise_workspace", c_int64, c_int32, c_int32, c_int32)
+    sig("cbm_b200_orthogonalise", c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32,
+        c_float, c_void_p, c_int64, c_void_p)
+    sig("cbm_b200_orthogonal_step_workspace", c_int64, c_void_p, c_int32)
+    sig("cbm_b200_orthogonal_step", c_int32, c_void_p, c_int32, c_float, c_float, c_int32, c_float, c_int32, c_float, c_void_p, c_int64,
+        c_void_p)
     _lib = L
     return L
 

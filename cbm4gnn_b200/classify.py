@@ -1,0 +1,95 @@
+"""What the logits of a stack are turned into: class log probabilities, their entropy and the most probable classes.
+
+``class_log_probs(logits, labels, top)`` gives for every row the log probability of its label, the entropy of the row's
+distribution and the ``top`` most probable classes with their log probabilities, from one pass over the logits, and is
+differentiable in them.  The reference stops at the logits (benchmark/parallel/benchmark_gcn_cpu.py:92-103 sums them).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .dense import _call, _ld, _rows
+from .norm import TYPES, rows_like
+
+MAX_TOP = 32  # include/cbm_b200.h, CBM_B200_MAX_TOP
+
+
+class ClassLogProbs(NamedTuple):
+    log_prob: torch.Tensor        # [N] fp32: of each row's label, 0 where the label is negative
+    entropy: torch.Tensor         # [N] fp32
+    top_log_probs: torch.Tensor   # [N, top] fp32, falling
+    top_classes: torch.Tensor     # [N, top] int64; of equal logits the lower class comes first
+
+
+class _ClassLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top):
+        x, n, c = _rows(logits), logits.size(0), logits.size(1)
+        labels = labels.contiguous()
+        new = dict(dtype=torch.float32, device=x.device)
+        log_prob, entropy, stats = torch.empty(n, **new), torch.empty(n, **new), torch.empty((n, 2), **new)
+        best, classes = torch.empty((n, top), **new), torch.empty((n, top), dtype=torch.int64, device=x.device)
+        _call("cbm_b200_class_log_probs", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(),
+              int(labels.dtype == torch.int64), n, c, top, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), best.data_ptr(),
+              classes.data_ptr())
+        ctx.save_for_backward(x, labels, stats, entropy, classes)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(classes)
+        return log_prob, entropy, best, classes
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log, g_entropy, g_top, _):
+        x, labels, stats, entropy, classes = ctx.saved_tensors
+        x, labels, stats, entropy, classes = _rows(x), labels.contiguous(), stats.contiguous(), entropy.contiguous(), classes.contiguous()
+        given = [None if g is None else g.contiguous() for g in (g_log, g_entropy, g_top)]
+        n, c = x.size(0), x.size(1)
+        gx = rows_like(x)
+        _call("cbm_b200_class_log_probs_grad", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(),
+              int(labels.dtype == torch.int64), n, c, classes.size(1), stats.data_ptr(), entropy.data_ptr(), classes.data_ptr(),
+              *(None if g is None else g.data_ptr() for g in given), gx.data_ptr(), _ld(gx))
+        return gx, None, None
+
+
+def _on_host(logits, labels, top):
+    """The same by torch's elementary operations, for CPU tensors."""
+    x = logits.float()
+    c = x.size(1)
+    m = x.detach().max(dim=1, keepdim=True).values
+    closed = m == -torch.inf
+    d = torch.where(closed, 0.0, x) - torch.where(closed, 0.0, m)
+    lp = d - torch.exp(d).sum(1, keepdim=True).log()
+    p = torch.exp(lp)
+    entropy = torch.where(closed[:, 0], 0.0, -(p * torch.where(p > 0, lp, 0.0)).sum(1))
+    lp = torch.where(closed, -torch.inf, lp)
+    known = labels >= 0
+    log_prob = torch.where(known, lp.gather(1, labels.long().clamp(0, c - 1)[:, None])[:, 0], 0.0)
+    log_prob = torch.where(labels >= c, torch.nan, log_prob)
+    best = torch.sort(x.detach(), dim=1, descending=True, stable=True).indices[:, :top]
+    return ClassLogProbs(log_prob, entropy, lp.gather(1, best), best)
+
+
+def class_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0) -> ClassLogProbs:
+    """For every row of ``logits`` [N, C] (fp32, bf16 or fp16; rows at any pitch): the log probability of its class
+    ``labels`` [N] (int64 or int32), the entropy of the row and its ``top`` most probable classes (0 to 32).
+
+    A negative label stands for none: log probability 0, no gradient.  One of C or more gives NaN.  A logit of -inf closes a
+    class; a row without an open class has log probabilities -inf, entropy 0 and no gradient.  A row with NaN or +inf is
+    NaN throughout.  Differentiable once in ``logits``, through all three results.
+    """
+    if logits.dim() != 2 or logits.size(1) < 1 or labels.shape != logits.shape[:1]:
+        raise RuntimeError(f"class log probabilities: shape mismatch, logits of {tuple(logits.shape)} and labels of {tuple(labels.shape)}")
+    if logits.dtype not in TYPES:
+        raise RuntimeError(f"class log probabilities: fp32, bf16 or fp16 logits expected, not {logits.dtype}")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"class log probabilities: int64 or int32 labels expected, not {labels.dtype}")
+    if labels.device != logits.device:
+        raise RuntimeError(f"class log probabilities: logits on {logits.device} and labels on {labels.device}")
+    if not 0 <= top <= min(MAX_TOP, logits.size(1)):
+        raise ValueError(f"top must be between 0 and {min(MAX_TOP, logits.size(1))}")
+    if not logits.is_cuda:
+        return _on_host(logits, labels, top)
+    return ClassLogProbs(*_ClassLogProbs.apply(logits, labels, int(top)))

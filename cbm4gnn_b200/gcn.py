@@ -16,8 +16,10 @@ import torch
 from torch import nn
 from torch.nn.modules.module import _has_any_global_hook
 
+from .classify import ClassLogProbs, class_log_probs
 from .dense import linear, linear_relu
 from .message_passing import CBMCudaMessagePassing
+from .norm import GroupNorm
 from .stack import run_stack
 
 
@@ -83,13 +85,21 @@ class CBMParallelTorchCSRSparseMatrixGCN(CBMCudaGCN):
 
 
 class GCNModel(nn.Module):
-    """``len(widths) - 1`` GCN layers with ReLU between them, sharing one CBM structure."""
+    """``len(widths) - 1`` GCN layers with ReLU between them, sharing one CBM structure.
 
-    def __init__(self, widths, structure=None, alpha: int = 2):
+    ``norm_groups``: a group norm of that many groups of channels in front of the activation between two layers, which
+    ``activation`` ("relu" or "silu") names; its samples are the graphs that ``forward`` is given by ``ptr``, or the whole
+    matrix."""
+
+    def __init__(self, widths, structure=None, alpha: int = 2, norm_groups: int | None = None, activation: str = "relu"):
         super().__init__()
         if len(widths) < 3:
             raise ValueError("Number of layers must be at least 2")
+        if activation not in ("relu", "silu") or (activation != "relu" and norm_groups is None):
+            raise ValueError("activation must be 'relu', or 'silu' behind a group norm")
         self.layers = nn.ModuleList(CBMCudaGCN(a, b, alpha=alpha) for a, b in zip(widths[:-1], widths[1:]))
+        self.norms = None if norm_groups is None else nn.ModuleList(
+            GroupNorm(norm_groups, width, activation=activation) for width in widths[1:-1])
         if structure is not None:
             self.share(structure)
 
@@ -101,10 +111,18 @@ class GCNModel(nn.Module):
         for layer in self.layers:
             layer.cached_a_t = structure
 
-    def forward(self, x, edge_index):
+    def forward(self, x, edge_index, ptr=None):
         """Layers of this library's own class run as one step (stack.py); where one was replaced, derived from,
-        given hooks (of its own or for all modules) or told to go by two steps, or off the GPU, layer by layer."""
+        given hooks (of its own or for all modules) or told to go by two steps, off the GPU, or with norms between
+        them, layer by layer.  ``ptr``: the rows ``ptr[s] .. ptr[s + 1]`` are a graph, for the norms."""
         layers = list(self.layers)
+        norms = getattr(self, "norms", None)  # (a model that was stored before there were any)
+        if norms is not None:
+            for layer, norm in zip(layers, norms):
+                x = norm(layer(x, edge_index), ptr)
+            return layers[-1](x, edge_index)
+        if ptr is not None:
+            raise ValueError("ptr is for the norms of a model with norm_groups")
         if x.is_cuda and x.dtype == torch.float32 and not _has_any_global_hook() and all(map(_plain, layers)):
             steps, weights = [], []
             for layer in layers:
@@ -116,6 +134,11 @@ class GCNModel(nn.Module):
         for i, layer in enumerate(layers):
             x = layer(x, edge_index, relu=i < last)
         return x
+
+    def log_probs(self, x, edge_index, labels, top: int = 0, ptr=None) -> ClassLogProbs:
+        """Log probability of every node's label by the model's logits, their entropy and the ``top`` most probable classes."""
+        logits = self(x, edge_index) if ptr is None else self(x, edge_index, ptr)
+        return class_log_probs(logits, labels, top)
 
 
 def _plain(layer) -> bool:

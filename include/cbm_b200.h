@@ -359,6 +359,80 @@ double cbm_b200_probe_l2_read_gbps(int32_t device);
 int cbm_b200_spmm_update_static(cbm_b200_plan* p, const float* x, int64_t ldx, float* y,
                                 int64_t ldy, int32_t f, int32_t normalized, void* stream);
 
+/* --------------------------------------------------------------------------------------------
+ * Operators around a stack of layers (the reference stops at the logits and has none of them).  `type`:
+ * CBM_B200_FP32, _BF16 or _FP16, of the operands that are declared void.  Launches are asynchronous on
+ * `stream`; nothing is allocated, kept or synchronised; every call may be captured.
+ *
+ * cbm_b200_class_log_probs       for every row of logits [dev, n_rows x n_classes, leading dimension ld]: the log
+ *                                probability of its label, the entropy of the row, and its `top` most probable
+ *                                classes with their log probabilities (equal logits: lower class first; top <= n_classes).
+ *                                labels [dev]: int64 where wide_labels, else int32; negative: none (log probability 0);
+ *                                n_classes or more: NaN.  stats [dev, 2 x n_rows] is for the gradient.
+ *                                top_log_prob, top_class [dev, n_rows x top].
+ * cbm_b200_class_log_probs_grad  dx [dev, type of the logits] from the gradients of log_prob [n_rows], entropy [n_rows] and
+ *                                top_log_prob [n_rows x top], of which any may be NULL; stats, entropy and top_class as the
+ *                                call above left them.
+ * ------------------------------------------------------------------------------------------ */
+#define CBM_B200_FP32 0
+#define CBM_B200_BF16 1
+#define CBM_B200_FP16 2
+#define CBM_B200_MAX_TOP 32
+int cbm_b200_class_log_probs(const void* logits, int64_t ld, int32_t type, const void* labels, int32_t wide_labels,
+                             int64_t n_rows, int32_t n_classes, int32_t top, float* log_prob, float* entropy,
+                             float* stats, float* top_log_prob, int64_t* top_class, void* stream);
+int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int32_t type, const void* labels, int32_t wide_labels,
+                                  int64_t n_rows, int32_t n_classes, int32_t top, const float* stats,
+                                  const float* entropy, const int64_t* top_class, const float* g_log_prob,
+                                  const float* g_entropy, const float* g_top, void* dx, int64_t lddx, void* stream);
+
+/* cbm_b200_group_norm       y = act(weight (x - mean) / sqrt(var + eps) + bias) for rows x [dev, n_rows x channels] in n_samples
+ *                           samples and `groups` equal ranges of channels; mean and variance of each sample's group.  The
+ *                           samples are the rows ptr[s] .. ptr[s + 1] (ptr [dev], n_samples + 1 entries, rising; kept inside the
+ *                           rows there are), or rows_each rows each where ptr is NULL.  Rows of no sample get 0.  weight and
+ *                           bias [dev, channels], fp32 where wide_params, else of `type`; NULL for 1 and 0.  mean and rstd
+ *                           [dev, n_samples x groups] for the gradient, both NULL where none follows.
+ * cbm_b200_group_norm_grad  gx, and gw and gb [dev, channels] (NULL: not wanted).
+ * cbm_b200_group_norm_workspace  bytes of workspace [dev] of either (`gradient` 0 or 1); n_samples negative: without ptr. */
+#define CBM_B200_ACT_NONE 0
+#define CBM_B200_ACT_RELU 1
+#define CBM_B200_ACT_SILU 2
+int64_t cbm_b200_group_norm_workspace(int64_t n_rows, int64_t n_samples, int32_t channels, int32_t groups, int32_t gradient);
+int cbm_b200_group_norm(const void* x, int64_t ldx, int32_t type, int64_t n_rows, int32_t channels, int32_t groups,
+                        const int64_t* ptr, int64_t n_samples, int64_t rows_each, const void* weight, const void* bias,
+                        int32_t wide_params, float eps, int32_t activation, void* y, int64_t ldy, float* mean,
+                        float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* gy, int64_t ldgy, int32_t type, int64_t n_rows,
+                             int32_t channels, int32_t groups, const int64_t* ptr, int64_t n_samples, int64_t rows_each,
+                             const void* weight, const void* bias, int32_t wide_params, int32_t activation, float* mean,
+                             float* rstd, void* gx, int64_t ldgx, float* gw, float* gb, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* cbm_b200_orthogonalise     out = U orthogonalised: X = U / (|U| + eps), then `steps` times A = X X^T,
+ *                            X <- a X + (b A + c A A) X with (a, b, c) = (3.4445, -4.7750, 2.0315); taller matrices are turned.
+ *                            `batch` matrices of rows x cols [dev], next_u and next_out floats apart.
+ * cbm_b200_orthogonal_step   for each of `count` weights [dev], in place: m <- momentum m + g;
+ *                            U = g + momentum m (nesterov) or m;
+ *                            w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalised(U).
+ *                            `of` is [host] and read before the call returns.
+ * Workspaces [dev] of the sizes given by the two functions; calls that may overlap must not share one. */
+#define CBM_B200_MAX_STEPS 64
+typedef struct {
+    float* w;
+    const float* g;
+    float* m;
+    int64_t ldw, ldg, ldm;
+    int32_t rows, cols;
+} cbm_b200_update_of;
+int64_t cbm_b200_orthogonalise_workspace(int32_t batch, int32_t rows, int32_t cols);
+int cbm_b200_orthogonalise(const float* u, int64_t ldu, int64_t next_u, float* out, int64_t ldout, int64_t next_out,
+                           int32_t batch, int32_t rows, int32_t cols, int32_t steps, float eps, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int64_t cbm_b200_orthogonal_step_workspace(const cbm_b200_update_of* of, int32_t count);
+int cbm_b200_orthogonal_step(const cbm_b200_update_of* of, int32_t count, float lr, float momentum, int32_t nesterov,
+                             float weight_decay, int32_t steps, float eps, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif
