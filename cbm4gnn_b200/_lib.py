@@ -245,7 +245,8 @@ def lib() -> ctypes.CDLL:
     sig("cbm_b200_group_norm", c_int32, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p,
         c_void_p, c_int32, c_float, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p)
     sig("cbm_b200_group_norm_grad", c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int64,
-        c_int64, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p)
+        c_int64, c_void_p, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
+        c_void_p)
     sig("cbm_b200_orthogonalise_workspace", c_int64, c_int32, c_int32, c_int32)
     sig("cbm_b200_orthogonalise", c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32,
         c_float, c_void_p, c_int64, c_void_p)

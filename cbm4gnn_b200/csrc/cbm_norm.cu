@@ -3,17 +3,30 @@
 // A sample is a range of rows (a graph), a group a range of channels.  With mean and r = 1 / sqrt(var + eps) over the values of
 // a sample's group:  xh = (x - mean) r,  z = w xh + b,  y = act(z).
 // Gradients, with g = gy act'(z) and u = w g:  gb = sum g,  gw = sum g xh,  gx = r (u - mean(u) - xh mean(u xh)).
+//
+// What bounds all of it is memory: x is read and y written once, x and gy are read and gx written once.  Three ways:
+//   * Samples of one row: lanes hold their part of a group in registers; nothing is read twice, and the gradient computes the
+//     statistics anew instead of reading them.
+//   * Samples of up to a tile's rows: a team of threads reads a sample, joins its sums in shared memory and reads it again, out of L1 or
+//     L2, to write the results.  Tiles end where samples do, so that each of these is one team's.
+//   * Longer samples: every tile leaves a partial result, one warp to a group joins them in a fixed order, and a third kernel
+//     goes over the rows again, from their ends, which L2 still holds.
+// Means and squares around them are kept for every few rows and joined (mean and sum of squares around it of two parts give those of
+// both), so that a mean far from 0 costs no digits; no sum depends on the order in which blocks run.
 #include "cbm_common.h"
 #include "cbm_launch.cuh"
 #include "cbm_values.cuh"
 
 #include <string>
+#include <type_traits>
 
 namespace {
 
 using u32 = uint32_t;
+using u64 = unsigned long long;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, SMS = 148;
+constexpr u32 FULL = 0xffffffffu;
 
 struct Params {
     const void *x, *gy;
@@ -25,25 +38,20 @@ struct Params {
     void* y;  // or gx
     float *mean, *r;
     float *gw, *gb;
+    // tiles
+    int64_t tile, tiles;        // rows to a tile; tiles
+    int team, slab_groups, lanes;    // threads of a team; groups of a column slab; threads of a group
+    float2 *pieces, *joined;    // [2][groups][tiles], [tiles][groups]
+    float2* channels;           // [tiles][c]: sums of g xh and g
+    int64_t parts;              // of `channels`
 };
-
-// Rows [first, last) of a sample; what a pointer array says is kept inside the rows there are.
-__device__ __forceinline__ void rows_of(const Params& p, int64_t s, int64_t& first, int64_t& last) {
-    if (p.ptr) {
-        first = min(max(p.ptr[s], (int64_t)0), p.n_rows);
-        last = min(max(p.ptr[s + 1], first), p.n_rows);
-    } else {
-        first = s * p.rows_each;
-        last = first + p.rows_each;
-    }
-}
 
 template <class T>
 __device__ __forceinline__ float param(const void* w, int wide, int c, float none) {
     return !w ? none : wide ? static_cast<const float*>(w)[c] : cbm::widen(static_cast<const T*>(w)[c]);
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 __device__ __forceinline__ float activated(float z, int act) {
     if (act == CBM_B200_ACT_RELU) return z <= 0.f ? 0.f : z;  // NaN passes
     return act == CBM_B200_ACT_SILU ? z * sigmoid(z) : z;
@@ -55,10 +63,564 @@ __device__ __forceinline__ float slope(float z, int act) {
     return s * (1.f + z * (1.f - s));
 }
 
+// The E values of a group that fall to a thread in each row.  Where rows and groups allow it they are one vector of up to 16 bytes; else
+// (STRIDED) they lie `lanes` values apart, so that neighbouring threads read neighbouring values, and the last may be missing.
+template <class T, int E, bool STRIDED>
+struct Values {
+    union {
+        T v[E];
+        std::conditional_t<sizeof(T) * E == 16, uint4, std::conditional_t<sizeof(T) * E == 8, uint2, std::conditional_t<sizeof(T) * E == 4, u32, uint16_t>>> bits;
+    };
+    __device__ Values() {}
+    __device__ __forceinline__ void load(const T* p, int lanes, int there) {
+        if constexpr (STRIDED) {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (i < there) v[i] = p[i * lanes];
+        } else {
+            bits = *reinterpret_cast<const decltype(bits)*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T* p, int lanes, int there) const {
+        if constexpr (STRIDED) {
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (i < there) p[i * lanes] = v[i];
+        } else {
+            *reinterpret_cast<decltype(bits)*>(p) = bits;
+        }
+    }
+};
+// Whether a thread has an i-th value.
+template <bool STRIDED>
+__device__ __forceinline__ bool has(int i, int there) {
+    return !STRIDED || i < there;
+}
+template <int E, bool STRIDED>
+__device__ __forceinline__ int values_of(int lane, int lanes, int width) {
+    return STRIDED ? (width - lane + lanes - 1) / lanes : E;
+}
+
+// Sum over `lanes` neighbouring lanes, a power of two.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+}
+
+// ---- samples of one row ---------------------------------------------------------------------------
+// The threads of a group (of up to 32: padded to a power of two; of more: to whole warps) hold its values in registers.  A thread's
+// channels stay the same from row to row, so that its weights are fetched once.
+struct RowShape {
+    int shift;           // threads of a group, with padding: 1 << shift, or 32 times `warps`
+    int warps;           // 0: up to 32 threads
+    int slots, at_once;  // threads of a slab's row, rows of a block
+    __host__ __device__ int padded() const { return warps ? 32 * warps : 1 << shift; }
+};
+
+// Sums of two values over a group's threads.
+__device__ __forceinline__ float2 group_sum(float2 v, const RowShape& h, float2* s_warp) {
+    if (!h.warps) return float2{lanes_sum(v.x, 1 << h.shift), lanes_sum(v.y, 1 << h.shift)};
+    v = float2{lanes_sum(v.x, 32), lanes_sum(v.y, 32)};
+    const int warp = threadIdx.x >> 5, first = warp / h.warps * h.warps;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_warp[warp] = v;
+    __syncthreads();
+    v = s_warp[first];
+    for (int i = 1; i < h.warps; ++i) v.x += s_warp[first + i].x, v.y += s_warp[first + i].y;
+    return v;
+}
+
+template <class T, int E, bool STRIDED, bool GRAD>
+__global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowShape h) {
+    __shared__ float2 s_warp[32];
+    cbm::wait_before();
+    const int row_in = threadIdx.x / h.slots, slot = threadIdx.x % h.slots, lane = slot % h.padded();
+    const int group = blockIdx.y * p.slab_groups + slot / h.padded();
+    const bool used = row_in < h.at_once && lane < p.lanes && group < p.groups;
+    const int there = used ? values_of<E, STRIDED>(lane, p.lanes, p.width) : 0;
+    const int at = group * p.width + (STRIDED ? lane : lane * E), stride = STRIDED ? p.lanes : 1;
+    float w[E], b[E], gw[E], gb[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        w[i] = i < there ? param<T>(p.w, p.wide_params, at + i * stride, 1.f) : 0.f;
+        b[i] = i < there ? param<T>(p.b, p.wide_params, at + i * stride, 0.f) : 0.f;
+        gw[i] = gb[i] = 0.f;
+    }
+    const float share = 1.f / (float)p.width;
+    const int64_t step = (int64_t)gridDim.x * h.at_once;
+    using V = Values<T, E, STRIDED>;
+    V xv, gv;
+    auto fetch = [&](int64_t row) {
+        if (used && row < p.n_rows) {
+            xv.load(static_cast<const T*>(p.x) + row * p.ldx + at, p.lanes, there);
+            if (GRAD) gv.load(static_cast<const T*>(p.gy) + row * p.ldgy + at, p.lanes, there);
+        }
+    };
+    int64_t row = (int64_t)blockIdx.x * h.at_once + row_in;
+    fetch(row);
+    // (all threads of a block take the same number of turns)
+    for (int64_t first = (int64_t)blockIdx.x * h.at_once; first < p.n_rows; first += step, row += step) {
+        const int now = row < p.n_rows ? there : 0;
+        float x[E], u[E];
+        float2 s{0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = i < now ? cbm::widen(xv.v[i]) : 0.f;
+            if (GRAD) u[i] = i < now ? cbm::widen(gv.v[i]) : 0.f;
+            s.x += x[i];
+        }
+        fetch(row + step);  // on its way meanwhile
+        const float mean = group_sum(s, h, s_warp).x * share;
+        s.x = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = i < now ? x[i] - mean : 0.f;
+            s.x += x[i] * x[i];
+        }
+        const float r = rsqrtf(group_sum(s, h, s_warp).x * share + p.eps);
+        V out;
+        if constexpr (!GRAD) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(activated(x[i] * (r * w[i]) + b[i], p.act));
+        } else {
+            s.x = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                x[i] *= r;
+                const float g = u[i] * slope(x[i] * w[i] + b[i], p.act);
+                gw[i] += g * x[i];
+                gb[i] += g;
+                u[i] = g * w[i];
+                s.x += u[i];
+                s.y += u[i] * x[i];
+            }
+            s = group_sum(s, h, s_warp);
+#pragma unroll
+            for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(r * (u[i] - s.x * share - x[i] * (s.y * share)));
+        }
+        if (now) out.store(static_cast<T*>(p.y) + row * p.ldy + at, p.lanes, there);
+    }
+    if constexpr (GRAD) {
+        if (!p.channels) return;
+        // the block's rows, one after the other
+        extern __shared__ float2 s_sum[];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            __syncthreads();
+            s_sum[threadIdx.x] = float2{gw[i], gb[i]};
+            __syncthreads();
+            if (row_in == 0 && i < there) {
+                float2 all = s_sum[slot];
+                for (int q = 1; q < h.at_once; ++q) {
+                    const float2 one = s_sum[q * h.slots + slot];
+                    all.x += one.x, all.y += one.y;
+                }
+                p.channels[(int64_t)blockIdx.x * p.c + at + i * stride] = all;
+            }
+        }
+    }
+}
+
+// ---- samples of several rows ----------------------------------------------------------------------
+// Row at which sample s starts; what a pointer array says is kept inside the rows there are.
+__device__ __forceinline__ int64_t start_of(const Params& p, int64_t s) {
+    return p.ptr ? min(max(p.ptr[s], (int64_t)0), p.n_rows) : s * p.rows_each;
+}
+// The last sample that starts at `row` or before it, -1: none.  The lanes of a warp try 32 places at a time.
+__device__ __forceinline__ int64_t sample_at(const Params& p, int64_t row) {
+    if (!p.ptr) return p.rows_each ? min(row / p.rows_each, p.n_samples - 1) : p.n_samples - 1;
+    const int lane = threadIdx.x & 31;
+    int64_t lo = 0, hi = p.n_samples + 1;  // entries before lo are <= row, those from hi on are larger
+    while (lo < hi) {
+        const int64_t each = (hi - lo + 31) / 32, probe = lo + each * lane + each - 1;
+        const bool below = probe < hi && p.ptr[probe] <= row;
+        const int n = __popc(__ballot_sync(FULL, below));
+        const int64_t from = lo;
+        lo = min(from + each * n, hi);
+        hi = min(hi, from + each * (n + 1) - 1);
+        if (hi < lo) hi = lo;
+    }
+    return lo - 1;
+}
+// Where the tile that should start at `row` does: samples that are no longer than a tile are not cut.
+__device__ __forceinline__ int64_t tile_start(const Params& p, int64_t row) {
+    if (row >= p.n_rows) return p.n_rows;
+    const int64_t s = sample_at(p, row);
+    if (s < 0 || s >= p.n_samples) return row;
+    const int64_t a = start_of(p, s), e = start_of(p, s + 1);
+    return row < e && e - a <= p.tile ? a : row;
+}
+
+struct Team {
+    int id, thread, size;              // of the block's; of the team's
+    int groups, vectors, at_once;      // of the slab; threads of its rows, rows at once
+    int group0, row_in, group, lane;   // this thread's; row_in >= at_once: none
+    int channel, there;                // first of its values, and how many
+    __device__ __forceinline__ Team(const Params& p, int E, bool strided) {
+        size = p.team;
+        id = threadIdx.x / size, thread = threadIdx.x % size;
+        group0 = blockIdx.y * p.slab_groups;
+        groups = min(p.slab_groups, p.groups - group0);
+        vectors = groups * p.lanes;
+        at_once = size / vectors;
+        row_in = thread / vectors;
+        group = group0 + thread % vectors / p.lanes, lane = thread % p.lanes;
+        if (row_in >= at_once) group = group0, lane = 0;
+        else lane = thread % vectors % p.lanes;
+        channel = group * p.width + (strided ? lane : lane * E);
+        there = strided ? (p.width - lane + p.lanes - 1) / p.lanes : E;
+    }
+    __device__ __forceinline__ bool on() const { return row_in < at_once; }
+    __device__ __forceinline__ void sync() const {
+        if (size == 32) __syncwarp();
+        else asm volatile("barrier.sync %0, %1;" ::"r"(id + 1), "r"(size) : "memory");
+    }
+};
+
+// Joins what the threads of a team found in `rows` rows into one result for each group.  f(group, sum of the two values) is called
+// by a lane for each group.  MEANS: the values are the mean over a thread's values of all its rows and the squares around it.
+template <bool MEANS, int E, bool STRIDED, class F>
+__device__ __forceinline__ void join_groups(const Params& p, const Team& t, const float2* part, int rows, F&& f) {
+    const int warp = t.thread >> 5, lane = t.thread & 31, entries = min(t.at_once, rows) * p.lanes;
+    for (int g = warp; g < t.groups; g += t.size >> 5) {
+        const float2* first = part + g * p.lanes;
+        if constexpr (MEANS) {
+            const float ref = first[0].x;
+            // f(what a thread left, how many values it is of)
+            auto each = [&](auto&& f) {
+                for (int i = lane; i < entries; i += 32) {
+                    const int r = i / p.lanes, l = i - r * p.lanes, n = (rows - r + t.at_once - 1) / t.at_once;
+                    f(first[r * t.vectors + l], (float)(n * values_of<E, STRIDED>(l, p.lanes, p.width)));
+                }
+            };
+            float s = 0.f;
+            each([&](float2 one, float n) { s += n * (one.x - ref); });
+            const float mean = ref + lanes_sum(s, 32) / ((float)rows * (float)p.width);
+            s = 0.f;
+            each([&](float2 one, float n) { s += one.y + n * (one.x - mean) * (one.x - mean); });
+            s = lanes_sum(s, 32);
+            if (lane == 0) f(g, float2{mean, s});
+        } else {
+            float2 s{0.f, 0.f};
+            for (int i = lane; i < entries; i += 32) {
+                const int r = i / p.lanes;
+                const float2 one = first[r * t.vectors + i - r * p.lanes];
+                s.x += one.x, s.y += one.y;
+            }
+            s.x = lanes_sum(s.x, 32), s.y = lanes_sum(s.y, 32);
+            if (lane == 0) f(g, s);
+        }
+    }
+}
+
+// Rows [lo, hi) of a sample: y, or gx, from the statistics (mean, r) and, for the gradient, the means of u and u xh; from the last row
+// to the first where BACK.
+template <class T, int E, bool STRIDED, bool GRAD, bool BACK>
+__device__ __forceinline__ void write_rows(const Params& p, const Team& t, int64_t lo, int64_t hi, const float (&w)[E], const float (&b)[E],
+                                           float2 stat, float2 sums) {
+    const int64_t first = lo + t.row_in;
+    if (!t.on() || first >= hi) return;
+    const int64_t count = (hi - first + t.at_once - 1) / t.at_once;
+    constexpr int BATCH = E == 8 ? 2 : 4;
+    const int64_t begin = BACK ? first + (count - 1) * t.at_once : first, step = BACK ? -t.at_once : t.at_once;
+    const T *x = static_cast<const T*>(p.x) + t.channel + begin * p.ldx, *gy = static_cast<const T*>(p.gy) + t.channel + begin * p.ldgy;
+    T* y = static_cast<T*>(p.y) + t.channel + begin * p.ldy;
+    const int64_t dx = step * p.ldx, dg = step * p.ldgy, dy = step * p.ldy;
+    float rw[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) rw[i] = stat.y * w[i];
+    for (int64_t q = 0; q < count; q += BATCH) {
+        Values<T, E, STRIDED> v[BATCH], gv[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+            if (q + k < count) {
+                v[k].load(x, p.lanes, t.there), x += dx;
+                if (GRAD) gv[k].load(gy, p.lanes, t.there), gy += dg;
+            }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (q + k >= count) break;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float d = cbm::widen(v[k].v[i]) - stat.x;
+                const float z = d * rw[i] + b[i];
+                float out;
+                if constexpr (GRAD) {
+                    const float u = cbm::widen(gv[k].v[i]) * slope(z, p.act) * w[i];
+                    out = stat.y * (u - sums.x - d * stat.y * sums.y);
+                } else {
+                    out = activated(z, p.act);
+                }
+                v[k].v[i] = cbm::narrow<T>(out);
+            }
+            v[k].store(y, p.lanes, t.there), y += dy;
+        }
+    }
+}
+
+template <class T, int E, bool STRIDED>
+__device__ __forceinline__ void fetch_params(const Params& p, const Team& t, float (&w)[E], float (&b)[E]) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool on = t.on() && has<STRIDED>(i, t.there);
+        w[i] = on ? param<T>(p.w, p.wide_params, t.channel + i * (STRIDED ? p.lanes : 1), 1.f) : 0.f;
+        b[i] = on ? param<T>(p.b, p.wide_params, t.channel + i * (STRIDED ? p.lanes : 1), 0.f) : 0.f;
+    }
+}
+
+// Blocks of an SM: what their registers leave room for without spilling.
+constexpr int blocks_resident(int e, bool grad) { return e == 8 ? (grad ? 2 : 3) : e == 4 && grad ? 3 : 4; }
+
+// A team to a tile: samples that lie in it are done with, of longer ones their part is left in `pieces`.
+template <class T, int E, bool STRIDED, bool GRAD>
+__global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kernel(const Params p) {
+    __shared__ float2 s_part[THREADS], s_stat[THREADS];
+    __shared__ float2 s_channel[GRAD ? THREADS * E : 1];
+    cbm::wait_before();
+    const Team t(p, E, STRIDED);
+    const int64_t tile = (int64_t)blockIdx.x * (THREADS / p.team) + t.id;
+    if (tile >= p.tiles) return;
+    float2 *part = s_part + t.id * t.size, *stat = s_stat + t.id * t.size;
+    float w[E], b[E], gw[E], gb[E];
+    fetch_params<T, E, STRIDED>(p, t, w, b);
+#pragma unroll
+    for (int i = 0; i < E; ++i) gw[i] = gb[i] = 0.f;
+    const int64_t tb = tile_start(p, tile * p.tile), te = tile_start(p, (tile + 1) * p.tile);
+    const T *x = static_cast<const T*>(p.x) + t.channel, *gy = static_cast<const T*>(p.gy) + t.channel;
+    using V = Values<T, E, STRIDED>;
+    if (p.ptr && tb < te) {  // rows of no sample
+        const int64_t head = p.n_samples ? start_of(p, 0) : p.n_rows, tail = p.n_samples ? start_of(p, p.n_samples) : p.n_rows;
+        V none;
+#pragma unroll
+        for (int i = 0; i < E; ++i) none.v[i] = cbm::narrow<T>(0.f);
+        T* y = static_cast<T*>(p.y) + t.channel;
+        for (int64_t row = tb + t.row_in; t.on() && row < min(te, head); row += t.at_once) none.store(y + row * p.ldy, p.lanes, t.there);
+        for (int64_t row = max(tb, tail) + t.row_in; t.on() && row < te; row += t.at_once) none.store(y + row * p.ldy, p.lanes, t.there);
+    }
+    int64_t s = tb < te ? max(sample_at(p, tb), (int64_t)0) : p.n_samples;
+    int64_t a = s < p.n_samples ? start_of(p, s) : te, e;
+    for (; s < p.n_samples && a < te; ++s, a = e) {
+        e = start_of(p, s + 1);
+        const int64_t lo = max(a, tb), hi = min(e, te);
+        if (lo >= hi) continue;
+        const bool whole = e - a <= p.tile;
+        const int rows = (int)(hi - lo);  // (at most two tiles, which fit 31 bits)
+        constexpr int BATCH = GRAD && E == 8 ? 2 : 4;
+        float2 at{0.f, 0.f};
+        if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
+        float mean[E], m2[E];  // of each channel; for the gradient the sums of g xh and g
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
+        if (t.on()) {
+            const T *px = x + (lo + t.row_in) * p.ldx, *pg = gy + (lo + t.row_in) * p.ldgy;
+            const int64_t dx = t.at_once * p.ldx, dg = t.at_once * p.ldgy;
+            for (int left = (rows - t.row_in + t.at_once - 1) / t.at_once; left > 0; left -= BATCH) {
+                V v[BATCH], gv[BATCH];
+                const int have = min(BATCH, left);
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (k < have) {
+                        v[k].load(px, p.lanes, t.there), px += dx;
+                        if (GRAD) gv[k].load(pg, p.lanes, t.there), pg += dg;
+                    }
+                if constexpr (GRAD) {
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k)
+                        if (k < have)
+#pragma unroll
+                            for (int i = 0; i < E; ++i) {
+                                if (!has<STRIDED>(i, t.there)) break;
+                                const float xh = (cbm::widen(v[k].v[i]) - at.x) * at.y;
+                                const float g = cbm::widen(gv[k].v[i]) * slope(xh * w[i] + b[i], p.act);
+                                mean[i] += g * xh;
+                                m2[i] += g;
+                            }
+                } else {
+                    const float share = 1.f / (float)have, to_mean = (float)have / (float)(n + have), to_squares = (float)n * to_mean;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        if (!has<STRIDED>(i, t.there)) break;
+                        float sum = 0.f, squares = 0.f;
+#pragma unroll
+                        for (int k = 0; k < BATCH; ++k) sum += k < have ? cbm::widen(v[k].v[i]) : 0.f;
+                        const float here = sum * share;
+#pragma unroll
+                        for (int k = 0; k < BATCH; ++k) {
+                            const float d = k < have ? cbm::widen(v[k].v[i]) - here : 0.f;
+                            squares += d * d;
+                        }
+                        const float d = here - mean[i];
+                        mean[i] += d * to_mean;
+                        m2[i] += squares + d * d * to_squares;
+                    }
+                    n += have;
+                }
+            }
+            float2 mine{0.f, 0.f};
+            if constexpr (GRAD) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    mine.x += m2[i] * w[i];    // u
+                    mine.y += mean[i] * w[i];  // u xh
+                    gw[i] += mean[i];
+                    gb[i] += m2[i];
+                }
+            } else {
+                float shift = 0.f;
+#pragma unroll
+                for (int i = 1; i < E; ++i) shift += has<STRIDED>(i, t.there) ? mean[i] - mean[0] : 0.f;
+                mine.x = mean[0] + shift / (float)t.there;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (has<STRIDED>(i, t.there)) mine.y += m2[i] + (float)n * (mean[i] - mine.x) * (mean[i] - mine.x);
+            }
+            part[t.thread] = mine;
+        }
+        t.sync();
+        join_groups<!GRAD, E, STRIDED>(p, t, part, rows, [&](int g, float2 all) {
+            if (!whole) {
+                const int64_t slot = a > tile * p.tile ? 1 : 0;  // a longer sample that starts inside the tile is its second one
+                p.pieces[(slot * p.groups + t.group0 + g) * p.tiles + tile] = all;
+                return;
+            }
+            const float share = 1.f / ((float)rows * (float)p.width);
+            if constexpr (GRAD) {
+                stat[g] = float2{all.x * share, all.y * share};
+            } else {
+                const float r = rsqrtf(all.y * share + p.eps);
+                stat[g] = float2{all.x, r};
+                if (p.mean) {
+                    p.mean[s * p.groups + t.group0 + g] = all.x;
+                    p.r[s * p.groups + t.group0 + g] = r;
+                }
+            }
+        });
+        t.sync();
+        if (!whole) continue;
+        const float2 found = stat[t.group - t.group0];
+        write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, hi, w, b, GRAD ? at : found, found);
+    }
+    if constexpr (GRAD) {
+        if (!p.channels) return;
+        float2* mine = s_channel + (t.id * t.size) * E;
+#pragma unroll
+        for (int i = 0; i < E; ++i) mine[i * t.size + t.thread] = float2{gw[i], gb[i]};
+        t.sync();
+        if (t.row_in == 0)
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if (!has<STRIDED>(i, t.there)) break;
+                float2 all = mine[i * t.size + t.thread];
+                for (int q = 1; q < t.at_once; ++q) {
+                    const float2 one = mine[i * t.size + t.thread + q * t.vectors];
+                    all.x += one.x, all.y += one.y;
+                }
+                p.channels[tile * p.c + t.channel + i * (STRIDED ? p.lanes : 1)] = all;
+            }
+    }
+}
+
+// The pieces of each sample that is longer than a tile, by the block of the tile in which it starts, a warp to a group.  The blocks behind
+// those of the tiles add up the channels' sums, 32 each.
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(1024) join_kernel(const Params p, int64_t tiles) {
+    cbm::wait_before();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x < tiles) {
+        const int64_t tile = blockIdx.x, end = (tile + 1) * p.tile;
+        if (end > p.n_rows) return;
+        const int64_t s = sample_at(p, end - 1);
+        if (s < 0 || s >= p.n_samples) return;
+        const int64_t a = start_of(p, s), e = start_of(p, s + 1);
+        if (a < tile * p.tile || e - a <= p.tile) return;
+        const int64_t last = (e - 1) / p.tile;
+        const float count = (float)(e - a) * (float)p.width;
+        for (int g = warp; g < p.groups; g += 32) {
+            const float2* found = p.pieces + (int64_t)g * p.tiles;
+            // of the first tile it is the second piece unless the sample starts with the tile
+            auto piece = [&](int64_t q) { return found[(q == tile && a > tile * p.tile ? p.groups * p.tiles : 0) + q]; };
+            if constexpr (GRAD) {
+                float2 all{0.f, 0.f};
+                for (int64_t q = tile + lane; q <= last; q += 32) {
+                    const float2 one = piece(q);
+                    all.x += one.x, all.y += one.y;
+                }
+                all.x = lanes_sum(all.x, 32), all.y = lanes_sum(all.y, 32);
+                if (lane == 0) p.joined[tile * p.groups + g] = float2{all.x / count, all.y / count};
+            } else {
+                auto rows = [&](int64_t q) { return (float)(min(e, (q + 1) * p.tile) - max(a, q * p.tile)); };
+                const float ref = piece(tile).x;
+                float m = 0.f, squares = 0.f;
+#pragma unroll 4
+                for (int64_t q = tile + lane; q <= last; q += 32) m += rows(q) * (piece(q).x - ref);
+                const float mean = ref + lanes_sum(m, 32) / (float)(e - a);
+#pragma unroll 4
+                for (int64_t q = tile + lane; q <= last; q += 32) {
+                    const float2 one = piece(q);
+                    squares += one.y + rows(q) * (float)p.width * (one.x - mean) * (one.x - mean);
+                }
+                const float r = rsqrtf(lanes_sum(squares, 32) / count + p.eps);
+                if (lane == 0) {
+                    p.joined[tile * p.groups + g] = float2{mean, r};
+                    if (p.mean) {
+                        p.mean[s * p.groups + g] = mean;
+                        p.r[s * p.groups + g] = r;
+                    }
+                }
+            }
+        }
+    } else if constexpr (GRAD) {
+        __shared__ float2 s_sum[32][33];
+        const int c = (int)(blockIdx.x - tiles) * 32 + lane;
+        float2 all{0.f, 0.f};
+        if (c < p.c)
+#pragma unroll 4
+            for (int64_t q = warp; q < p.parts; q += 32) {
+                const float2 one = p.channels[q * p.c + c];
+                all.x += one.x, all.y += one.y;
+            }
+        s_sum[warp][lane] = all;
+        __syncthreads();
+        all = s_sum[lane][warp];
+        all.x = lanes_sum(all.x, 32), all.y = lanes_sum(all.y, 32);
+        const int mine = (int)(blockIdx.x - tiles) * 32 + warp;
+        if (lane == 0 && mine < p.c) {
+            if (p.gw) p.gw[mine] = all.x;
+            if (p.gb) p.gb[mine] = all.y;
+        }
+    }
+}
+
+// The rows of samples that are longer than a tile: at most two of them meet in one.
+template <class T, int E, bool STRIDED, bool GRAD>
+__global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) long_kernel(const Params p) {
+    cbm::wait_before();
+    const Team t(p, E, STRIDED);
+    const int64_t tile = (int64_t)blockIdx.x * (THREADS / p.team) + t.id;
+    if (tile >= p.tiles) return;
+    float w[E], b[E];
+    fetch_params<T, E, STRIDED>(p, t, w, b);
+    const int64_t begin = tile * p.tile, end = min(begin + p.tile, p.n_rows);
+    int64_t last = -1;
+    for (int k = 0; k < 2; ++k) {
+        const int64_t s = sample_at(p, k == 0 ? end - 1 : begin);
+        if (s < 0 || s >= p.n_samples || s == last) continue;
+        last = s;
+        const int64_t a = start_of(p, s), e = start_of(p, s + 1);
+        if (e - a <= p.tile || !t.on()) continue;
+        const int64_t lo = max(a, begin), hi = min(e, end);
+        const float2 found = p.joined[(a / p.tile) * p.groups + t.group];
+        float2 at = found;
+        if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
+        if (lo < hi) write_rows<T, E, STRIDED, GRAD, true>(p, t, lo, hi, w, b, at, found);
+    }
+}
+
+// ---- groups that are wider than a block -----------------------------------------------------------
 __device__ __forceinline__ float block_sum(float v) {
     __shared__ float part[THREADS / 32];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = lanes_sum(v, 32);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
@@ -68,98 +630,78 @@ __device__ __forceinline__ float block_sum(float v) {
     return s;
 }
 
-// A block to a sample's group.
-template <class T>
-__global__ void __launch_bounds__(THREADS) norm_kernel(const Params p) {
+// A block to a sample's group, value by value.
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
     cbm::wait_before();
     for (int64_t unit = blockIdx.x; unit < p.n_samples * p.groups; unit += gridDim.x) {
-        int64_t first, last;
-        rows_of(p, unit / p.groups, first, last);
+        const int64_t s = unit / p.groups, first = start_of(p, s), last = max(start_of(p, s + 1), first), count = (last - first) * p.width;
         const int c0 = (int)(unit % p.groups) * p.width;
-        const int64_t count = (last - first) * p.width;
-        const T* x = static_cast<const T*>(p.x);
-        float s = 0.f;
-        for (int64_t i = threadIdx.x; i < count; i += THREADS) s += cbm::widen(x[(first + i / p.width) * p.ldx + c0 + i % p.width]);
-        const float mean = block_sum(s) / (float)max(count, (int64_t)1);
-        s = 0.f;
-        for (int64_t i = threadIdx.x; i < count; i += THREADS) {
-            const float d = cbm::widen(x[(first + i / p.width) * p.ldx + c0 + i % p.width]) - mean;
-            s += d * d;
-        }
-        const float r = rsqrtf(block_sum(s) / (float)max(count, (int64_t)1) + p.eps);
-        for (int64_t i = threadIdx.x; i < count; i += THREADS) {
-            const int64_t row = first + i / p.width;
-            const int c = c0 + (int)(i % p.width);
-            const float z = (cbm::widen(x[row * p.ldx + c]) - mean) * r * param<T>(p.w, p.wide_params, c, 1.f) + param<T>(p.b, p.wide_params, c, 0.f);
-            static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(activated(z, p.act));
-        }
-        if (threadIdx.x == 0 && p.mean) {
-            p.mean[unit] = mean;
-            p.r[unit] = r;
-        }
-    }
-}
-
-template <class T>
-__global__ void __launch_bounds__(THREADS) norm_grad_kernel(const Params p) {
-    cbm::wait_before();
-    for (int64_t unit = blockIdx.x; unit < p.n_samples * p.groups; unit += gridDim.x) {
-        int64_t first, last;
-        rows_of(p, unit / p.groups, first, last);
-        const int c0 = (int)(unit % p.groups) * p.width;
-        const int64_t count = (last - first) * p.width;
-        const float mean = p.mean[unit], r = p.r[unit];
         const T *x = static_cast<const T*>(p.x), *gy = static_cast<const T*>(p.gy);
-        float su = 0.f, sux = 0.f;
-        for (int step = 0; step < 2; ++step) {
-            for (int64_t i = threadIdx.x; i < count; i += THREADS) {
-                const int64_t row = first + i / p.width;
-                const int c = c0 + (int)(i % p.width);
-                const float w = param<T>(p.w, p.wide_params, c, 1.f), xh = (cbm::widen(x[row * p.ldx + c]) - mean) * r;
-                const float u = cbm::widen(gy[row * p.ldgy + c]) * slope(xh * w + param<T>(p.b, p.wide_params, c, 0.f), p.act) * w;
-                if (step == 0) su += u, sux += u * xh;
-                else static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(r * (u - su - xh * sux));
-            }
-            if (step == 0) {
-                su = block_sum(su) / (float)max(count, (int64_t)1);
-                sux = block_sum(sux) / (float)max(count, (int64_t)1);
-            }
+        const float share = 1.f / (float)max(count, (int64_t)1);
+        // f(row, channel, value)
+        auto each = [&](auto&& f) {
+            for (int64_t row = first; row < last; ++row)
+                for (int c = threadIdx.x; c < p.width; c += THREADS) f(row, c0 + c, cbm::widen(x[row * p.ldx + c0 + c]));
+        };
+        float sum = 0.f;
+        each([&](int64_t, int, float v) { sum += v; });
+        const float mean = block_sum(sum) * share;
+        sum = 0.f;
+        each([&](int64_t, int, float v) { sum += (v - mean) * (v - mean); });
+        const float r = rsqrtf(block_sum(sum) * share + p.eps);
+        if constexpr (!GRAD) {
+            each([&](int64_t row, int c, float v) {
+                const float z = (v - mean) * (r * param<T>(p.w, p.wide_params, c, 1.f)) + param<T>(p.b, p.wide_params, c, 0.f);
+                static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(activated(z, p.act));
+            });
+            if (threadIdx.x == 0 && p.mean) p.mean[unit] = mean, p.r[unit] = r;
+        } else {
+            float su = 0.f, sux = 0.f;
+            auto u_of = [&](int64_t row, int c, float xh) {
+                const float w = param<T>(p.w, p.wide_params, c, 1.f);
+                return cbm::widen(gy[row * p.ldgy + c]) * slope(xh * w + param<T>(p.b, p.wide_params, c, 0.f), p.act) * w;
+            };
+            each([&](int64_t row, int c, float v) {
+                const float xh = (v - mean) * r, u = u_of(row, c, xh);
+                su += u, sux += u * xh;
+            });
+            su = block_sum(su) * share, sux = block_sum(sux) * share;
+            each([&](int64_t row, int c, float v) {
+                const float xh = (v - mean) * r;
+                static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(r * (u_of(row, c, xh) - su - xh * sux));
+            });
+            if (threadIdx.x == 0) p.joined[unit] = float2{mean, r};
         }
     }
 }
 
-// A block to a channel: the gradients of its weight and bias, over all samples.
+// Sums over ranges of rows of g xh and g, a thread to a channel; behind wide_kernel, with its statistics.
 template <class T>
-__global__ void __launch_bounds__(THREADS) norm_params_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS) wide_params_kernel(const Params p) {
     cbm::wait_before();
-    const int c = blockIdx.x, group = c / p.width;
+    const int c = blockIdx.y * THREADS + threadIdx.x;
+    if (c >= p.c) return;
     const float w = param<T>(p.w, p.wide_params, c, 1.f), b = param<T>(p.b, p.wide_params, c, 0.f);
-    float gw = 0.f, gb = 0.f;
-    for (int64_t s = 0; s < p.n_samples; ++s) {
-        int64_t first, last;
-        rows_of(p, s, first, last);
-        const float mean = p.mean[s * p.groups + group], r = p.r[s * p.groups + group];
-        for (int64_t row = first + threadIdx.x; row < last; row += THREADS) {
-            const float xh = (cbm::widen(static_cast<const T*>(p.x)[row * p.ldx + c]) - mean) * r;
+    float2 all{0.f, 0.f};
+    const int64_t each = (p.n_samples + p.parts - 1) / p.parts, to = min((blockIdx.x + 1) * each, p.n_samples);
+    for (int64_t s = blockIdx.x * each; s < to; ++s) {
+        const float2 at = p.joined[s * p.groups + c / p.width];
+        const int64_t last = start_of(p, s + 1);
+        for (int64_t row = start_of(p, s); row < last; ++row) {
+            const float xh = (cbm::widen(static_cast<const T*>(p.x)[row * p.ldx + c]) - at.x) * at.y;
             const float g = cbm::widen(static_cast<const T*>(p.gy)[row * p.ldgy + c]) * slope(xh * w + b, p.act);
-            gw += g * xh;
-            gb += g;
+            all.x += g * xh, all.y += g;
         }
     }
-    gw = block_sum(gw);
-    gb = block_sum(gb);
-    if (threadIdx.x == 0) {
-        if (p.gw) p.gw[c] = gw;
-        if (p.gb) p.gb[c] = gb;
-    }
+    p.channels[(int64_t)blockIdx.x * p.c + c] = all;
 }
 
 // Rows of no sample: 0.
 template <class T>
-__global__ void __launch_bounds__(THREADS) norm_outside_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS) outside_kernel(const Params p) {
     cbm::wait_before();
-    const int64_t head = p.n_samples ? min(max(p.ptr[0], (int64_t)0), p.n_rows) : p.n_rows;
-    const int64_t tail = p.n_samples ? min(max(p.ptr[p.n_samples], head), p.n_rows) : p.n_rows;
+    const int64_t head = p.n_samples ? start_of(p, 0) : p.n_rows, tail = p.n_samples ? max(start_of(p, p.n_samples), head) : p.n_rows;
     const int64_t outside = head + p.n_rows - tail;
     for (int64_t i = blockIdx.x; i < outside; i += gridDim.x) {
         T* to = static_cast<T*>(p.y) + (i < head ? i : i - head + tail) * p.ldy;
@@ -167,57 +709,206 @@ __global__ void __launch_bounds__(THREADS) norm_outside_kernel(const Params p) {
     }
 }
 
-int check(const char* who, const Params& p, int32_t type) {
-    const bool fits = p.n_rows >= 0 && p.n_samples >= 0 && p.c >= 1 && p.groups >= 1 && p.c % p.groups == 0 && p.ldx >= p.c && p.ldy >= p.c &&
-                      p.act >= 0 && p.act <= CBM_B200_ACT_SILU && type >= 0 && type <= CBM_B200_FP16 && p.eps >= 0.f &&
-                      (p.ptr || (p.rows_each >= 0 && (p.n_samples == 0 ? p.n_rows == 0 : p.n_rows % p.n_samples == 0 && p.n_rows / p.n_samples == p.rows_each)));
-    return fits ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes, type or activation");
-}
-
+// ---- host -----------------------------------------------------------------------------------------
 int launched(const char* who) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
-dim3 blocks_for(int64_t units) { return dim3((unsigned)(units < 148 * 32 ? units : 148 * 32)); }
+int check(const char* who, const Params& p, int32_t type) {
+    const bool fits = p.n_rows >= 0 && p.n_rows < ((int64_t)1 << 40) && p.n_samples >= 0 && p.c >= 1 && p.groups >= 1 && p.c % p.groups == 0 &&
+                      p.ldx >= p.c && p.ldy >= p.c && p.act >= 0 && p.act <= CBM_B200_ACT_SILU && type >= 0 && type <= CBM_B200_FP16 && p.eps >= 0.f &&
+                      (p.ptr || (p.rows_each >= 0 && (p.n_samples == 0 ? p.n_rows == 0 : p.n_rows % p.n_samples == 0 && p.n_rows / p.n_samples == p.rows_each)));
+    return fits ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes, type or activation");
+}
+
+enum Way { ROWS, TILES, WIDE };
+
+// The values of a row that fall to a thread: E of them, as one vector or (strided) as many threads of a group apart.
+struct Form {
+    int e;
+    bool strided;
+    int lanes(int width) const { return (width + e - 1) / e; }
+};
+
+// How a norm is computed, from its sizes and the form.
+struct Plan {
+    Way way;
+    Form form;
+    RowShape rows;
+    int64_t blocks;    // with ROWS
+    int lanes, team, slab_groups;
+    int64_t tile, tiles, parts;
+    bool joins;        // whether samples may be longer than a tile
+
+    Plan(int64_t n_rows, int64_t n_samples, bool ptr, int64_t rows_each, int c, int groups, Form f, bool grad) : form(f) {
+        const int width = c / groups;
+        joins = false;
+        tile = tiles = 0;
+        if (!ptr && rows_each == 1 && form.lanes(width) <= 1024) {
+            way = ROWS;
+            lanes = form.lanes(width);
+            rows.warps = lanes > 32 ? (lanes + 31) / 32 : 0;
+            for (rows.shift = 0; rows.shift < 5 && 1 << rows.shift < lanes;) ++rows.shift;
+            slab_groups = THREADS / rows.padded() < 1 ? 1 : THREADS / rows.padded() < groups ? THREADS / rows.padded() : groups;
+            rows.slots = slab_groups * rows.padded();
+            rows.at_once = rows.slots >= THREADS ? 1 : THREADS / rows.slots;
+            const int64_t turns = (n_rows + rows.at_once - 1) / rows.at_once;
+            const int64_t most = (int64_t)SMS * (2048 / threads()) / 2;  // (half of what an SM holds: their registers)
+            blocks = turns < most ? turns : most;
+            parts = blocks;
+            return;
+        }
+        if (form.lanes(width) > THREADS) form = Form{8, true};
+        lanes = form.lanes(width);
+        if (lanes > THREADS) {
+            way = WIDE;
+            parts = n_samples < SMS ? (n_samples > 0 ? n_samples : 1) : SMS;
+            return;
+        }
+        way = TILES;
+        slab_groups = THREADS / lanes < groups ? THREADS / lanes : groups;
+        // Four rows of a slab at once, at least a warp.
+        for (team = 32; team < THREADS && team < 4 * slab_groups * lanes;) team *= 2;
+        const int at_once = team / (slab_groups * lanes), slabs = (groups + slab_groups - 1) / slab_groups;
+        int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
+        if (teams < 1) teams = 1;
+        tile = (n_rows + teams - 1) / teams;
+        if (tile < 8 * at_once) tile = 8 * at_once;
+        tiles = (n_rows + tile - 1) / tile;
+        parts = tiles;
+        joins = ptr || rows_each > tile;
+    }
+    int threads() const { return (rows.slots * rows.at_once + 31) / 32 * 32; }
+    int64_t piece_bytes(int groups) const { return way == TILES && joins ? 8 * 3 * tiles * groups : 0; }
+    int64_t bytes(int64_t n_samples, int c, int groups, bool grad) const {
+        return (grad ? 8 * parts * c : 0) + piece_bytes(groups) + (way == WIDE && grad ? 8 * n_samples * groups : 0);
+    }
+};
+
+// Vectors of the largest power of two of values, up to 16 bytes, that divides a group's channels and at which all rows are aligned;
+// where that is one value, four strided ones (narrow groups: one).
+Form form_of(const Params& p, int size) {
+    int e = 16 / size;
+    auto aligned = [&](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % (e * size) == 0 && ld % e == 0; };
+    while (e > 1 && (p.width % e || !aligned(p.x, p.ldx) || !aligned(p.y, p.ldy) || (p.gy && !aligned(p.gy, p.ldgy)))) e /= 2;
+    return e > 1 ? Form{e, false} : Form{p.width > 2 ? 4 : 1, true};
+}
+
+// Calls f with the number of values and whether they are strided as constants.
+template <class T, class F>
+void with_form(Form form, F&& f) {
+    using Y = std::true_type;
+    using N = std::false_type;
+    if (form.strided) {
+        if (form.e == 1) f(std::integral_constant<int, 1>(), Y());
+        else if (form.e == 4) f(std::integral_constant<int, 4>(), Y());
+        else f(std::integral_constant<int, 8>(), Y());
+    } else {
+        if (form.e == 2) f(std::integral_constant<int, 2>(), N());
+        else if (form.e == 4) f(std::integral_constant<int, 4>(), N());
+        else if constexpr (sizeof(T) == 2) f(std::integral_constant<int, 8>(), N());
+    }
+}
+
+dim3 blocks_for(int64_t units) { return dim3((unsigned)(units < SMS * 32 ? (units > 0 ? units : 1) : SMS * 32)); }
+
+template <class T, bool GRAD>
+void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::Stream& on) {
+    const bool sums = GRAD && (p.gw || p.gb);
+    p.parts = p.n_rows ? plan.parts : 0;
+    if (sums) p.channels = reinterpret_cast<float2*>(workspace);
+    workspace += GRAD ? 8 * plan.parts * p.c : 0;
+    p.lanes = plan.lanes, p.slab_groups = plan.slab_groups, p.team = plan.team, p.tile = plan.tile, p.tiles = plan.tiles;
+    int64_t joins = 0;
+    if (p.n_rows == 0) {
+        // nothing but the sums of nothing
+    } else if (plan.way == ROWS) {
+        with_form<T>(plan.form, [&](auto e, auto strided) {
+            const unsigned threads = plan.threads();
+            const dim3 grid((unsigned)plan.blocks, (p.groups + p.slab_groups - 1) / p.slab_groups);
+            cbm::launch_next(rows_kernel<T, decltype(e)::value, decltype(strided)::value, GRAD>, grid, threads, sums ? 8 * threads : 0, on, p, plan.rows);
+        });
+    } else if (plan.way == TILES) {
+        p.pieces = reinterpret_cast<float2*>(workspace);
+        p.joined = p.pieces + 2 * p.tiles * p.groups;
+        const int per_block = THREADS / p.team;
+        const dim3 grid((unsigned)((p.tiles + per_block - 1) / per_block), (p.groups + p.slab_groups - 1) / p.slab_groups);
+        with_form<T>(plan.form, [&](auto e, auto strided) {
+            constexpr int E = decltype(e)::value;
+            constexpr bool STRIDED = decltype(strided)::value;
+            cbm::launch_next(tiles_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
+            if (!plan.joins) return;
+            joins = p.tiles;
+            cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)(joins + (sums ? (p.c + 31) / 32 : 0))), 1024, 0, on, p, joins);
+            cbm::launch_next(long_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
+        });
+    } else {
+        p.joined = reinterpret_cast<float2*>(workspace);
+        if (p.n_samples) cbm::launch_next(wide_kernel<T, GRAD>, blocks_for(p.n_samples * p.groups), THREADS, 0, on, p);
+        if (p.ptr) cbm::launch_next(outside_kernel<T>, blocks_for(p.n_rows), THREADS, 0, on, p);
+        if (sums) cbm::launch_next(wide_params_kernel<T>, dim3((unsigned)p.parts, (p.c + THREADS - 1) / THREADS), THREADS, 0, on, p);
+    }
+    if (sums && !joins) cbm::launch_next(join_kernel<T, true>, dim3((p.c + 31) / 32), 1024, 0, on, p, joins);
+}
+
+// Workspace of a call, whatever the type and the alignment of its rows.
+int64_t workspace_of(int64_t n_rows, int64_t n_samples, bool ptr, int64_t rows_each, int c, int groups, bool grad) {
+    static const Form forms[] = {{1, true}, {4, true}, {2, false}, {4, false}, {8, false}};
+    int64_t most = 0;
+    for (const Form f : forms) {
+        if (!f.strided && c / groups % f.e) continue;
+        const int64_t bytes = Plan(n_rows, n_samples, ptr, rows_each, c, groups, f, grad).bytes(n_samples, c, groups, grad);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
 
 }  // namespace
 
-extern "C" int64_t cbm_b200_group_norm_workspace(int64_t, int64_t, int32_t, int32_t, int32_t) { return 0; }
+extern "C" int64_t cbm_b200_group_norm_workspace(int64_t n_rows, int64_t n_samples, int32_t channels, int32_t groups, int32_t gradient) {
+    const bool ptr = n_samples >= 0;
+    const int64_t samples = ptr ? n_samples : -n_samples;
+    if (n_rows < 0 || channels < 1 || groups < 1 || channels % groups) return 0;
+    return workspace_of(n_rows, samples, ptr, ptr || samples == 0 ? 0 : n_rows / samples, channels, groups, gradient != 0);
+}
 
 extern "C" int cbm_b200_group_norm(const void* x, int64_t ldx, int32_t type, int64_t n_rows, int32_t channels, int32_t groups,
                                    const int64_t* ptr, int64_t n_samples, int64_t rows_each, const void* weight, const void* bias,
                                    int32_t wide_params, float eps, int32_t activation, void* y, int64_t ldy, float* mean, float* rstd,
-                                   void*, int64_t, void* stream) {
-    Params p{x, nullptr, weight, bias, ldx, 0, ldy, n_rows, n_samples, rows_each, ptr, channels, groups, groups > 0 ? channels / groups : 0,
-             activation, wide_params, eps, y, mean, rstd, nullptr, nullptr};
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+    Params p{};
+    p.x = x, p.w = weight, p.b = bias, p.ldx = ldx, p.ldy = ldy, p.n_rows = n_rows, p.n_samples = n_samples, p.rows_each = rows_each;
+    p.ptr = ptr, p.c = channels, p.groups = groups, p.width = groups > 0 ? channels / groups : 0, p.act = activation;
+    p.wide_params = wide_params, p.eps = eps, p.y = y, p.mean = mean, p.r = rstd;
     if (int rc = check("group_norm", p, type)) return rc;
     if (n_rows == 0) return CBM_B200_OK;
     if (!x || !y || !mean != !rstd) return cbm::fail(CBM_B200_ERR_ARG, "group_norm: NULL argument");
+    const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), false);
+    const int64_t need = plan.bytes(n_samples, channels, groups, false);
+    if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm: workspace too small");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
-    cbm::with_type(type, [&](auto t) {
-        using T = decltype(t);
-        if (n_samples) cbm::launch_next(norm_kernel<T>, blocks_for(n_samples * groups), THREADS, 0, on, p);
-        if (ptr) cbm::launch_next(norm_outside_kernel<T>, blocks_for(n_rows), THREADS, 0, on, p);
-    });
+    cbm::with_type(type, [&](auto t) { launch<decltype(t), false>(p, plan, static_cast<unsigned char*>(workspace), on); });
     return launched("group_norm");
 }
 
 extern "C" int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* gy, int64_t ldgy, int32_t type, int64_t n_rows,
                                         int32_t channels, int32_t groups, const int64_t* ptr, int64_t n_samples, int64_t rows_each,
-                                        const void* weight, const void* bias, int32_t wide_params, int32_t activation, float* mean,
-                                        float* rstd, void* gx, int64_t ldgx, float* gw, float* gb, void*, int64_t, void* stream) {
-    Params p{x, gy, weight, bias, ldx, ldgy, ldgx, n_rows, n_samples, rows_each, ptr, channels, groups, groups > 0 ? channels / groups : 0,
-             activation, wide_params, 0.f, gx, mean, rstd, gw, gb};
+                                        const void* weight, const void* bias, int32_t wide_params, float eps, int32_t activation,
+                                        float* mean, float* rstd, void* gx, int64_t ldgx, float* gw, float* gb, void* workspace,
+                                        int64_t workspace_bytes, void* stream) {
+    Params p{};
+    p.x = x, p.gy = gy, p.w = weight, p.b = bias, p.ldx = ldx, p.ldgy = ldgy, p.ldy = ldgx, p.n_rows = n_rows, p.n_samples = n_samples;
+    p.rows_each = rows_each, p.ptr = ptr, p.c = channels, p.groups = groups, p.width = groups > 0 ? channels / groups : 0, p.act = activation;
+    p.wide_params = wide_params, p.eps = eps, p.y = gx, p.mean = mean, p.r = rstd, p.gw = gw, p.gb = gb;
     if (int rc = check("group_norm_grad", p, type)) return rc;
     if (ldgy < channels) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: rows of the gradient overlap");
-    if ((n_samples && (!mean || !rstd)) || (n_rows && (!x || !gy || !gx))) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
+    if (n_rows && (!x || !gy || !gx)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
+    const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), true);
+    if (n_rows && plan.way == TILES && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
+    const int64_t need = plan.bytes(n_samples, channels, groups, true);
+    if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: workspace too small");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
-    cbm::with_type(type, [&](auto t) {
-        using T = decltype(t);
-        if (n_samples && n_rows) cbm::launch_next(norm_grad_kernel<T>, blocks_for(n_samples * groups), THREADS, 0, on, p);
-        if (ptr && n_rows) cbm::launch_next(norm_outside_kernel<T>, blocks_for(n_rows), THREADS, 0, on, p);
-        if (gw || gb) cbm::launch_next(norm_params_kernel<T>, dim3(channels), THREADS, 0, on, p);
-    });
+    cbm::with_type(type, [&](auto t) { launch<decltype(t), true>(p, plan, static_cast<unsigned char*>(workspace), on); });
     return launched("group_norm_grad");
 }

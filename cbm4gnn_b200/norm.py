@@ -38,7 +38,7 @@ class _GroupNorm(torch.autograd.Function):
         n, c = x.size(0), x.size(1)
         y = rows_like(x)
         mean = r = None
-        if keep:
+        if keep and (ptr is not None or rows_each != 1):  # (of single rows the gradient computes them anew)
             mean, r = (torch.empty((samples, groups), dtype=torch.float32, device=x.device) for _ in range(2))
         wide = int((weight if weight is not None else bias if bias is not None else x).dtype == torch.float32)
         space = _lib.lib().cbm_b200_group_norm_workspace(n, samples if ptr is not None else -samples, c, groups, 0)
@@ -47,7 +47,7 @@ class _GroupNorm(torch.autograd.Function):
               _data(weight), _data(bias), wide, eps, act, y.data_ptr(), _ld(y), _data(mean), _data(r), ws.data_ptr(), space)
         if keep:
             ctx.save_for_backward(x, weight, bias, ptr, mean, r)
-            ctx.sizes = samples, rows_each, groups, act, wide
+            ctx.sizes = samples, rows_each, groups, eps, act, wide
         return y
 
     @staticmethod
@@ -55,16 +55,16 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, gy):
         x, weight, bias, ptr, mean, r = ctx.saved_tensors
         # (a saved-tensor hook may hand them back in another layout)
-        x, gy, mean, r = _rows(x), _rows(gy), mean.contiguous(), r.contiguous()
-        weight, bias, ptr = (None if t is None else t.contiguous() for t in (weight, bias, ptr))
-        samples, rows_each, groups, act, wide = ctx.sizes
+        x, gy = _rows(x), _rows(gy)
+        weight, bias, ptr, mean, r = (None if t is None else t.contiguous() for t in (weight, bias, ptr, mean, r))
+        samples, rows_each, groups, eps, act, wide = ctx.sizes
         n, c = x.size(0), x.size(1)
         gx = rows_like(x)
         gw, gb = (torch.empty(c, dtype=torch.float32, device=x.device) if need else None for need in ctx.needs_input_grad[1:3])
         space = _lib.lib().cbm_b200_group_norm_workspace(n, samples if ptr is not None else -samples, c, groups, 1)
         ws = torch.empty(space, dtype=torch.uint8, device=x.device)
         _call("cbm_b200_group_norm_grad", x.get_device(), x.data_ptr(), _ld(x), gy.data_ptr(), _ld(gy), TYPES[x.dtype], n, c, groups,
-              _data(ptr), samples, rows_each, _data(weight), _data(bias), wide, act, mean.data_ptr(), r.data_ptr(), gx.data_ptr(), _ld(gx),
+              _data(ptr), samples, rows_each, _data(weight), _data(bias), wide, eps, act, _data(mean), _data(r), gx.data_ptr(), _ld(gx),
               _data(gw), _data(gb), ws.data_ptr(), space)
         if gw is not None:
             gw = gw.to(weight.dtype)

@@ -391,7 +391,8 @@ int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int32_t type, 
  *                           samples are the rows ptr[s] .. ptr[s + 1] (ptr [dev], n_samples + 1 entries, rising; kept inside the
  *                           rows there are), or rows_each rows each where ptr is NULL.  Rows of no sample get 0.  weight and
  *                           bias [dev, channels], fp32 where wide_params, else of `type`; NULL for 1 and 0.  mean and rstd
- *                           [dev, n_samples x groups] for the gradient, both NULL where none follows.
+ *                           [dev, n_samples x groups] for the gradient, both NULL where none follows.  (Where samples are one row
+ *                           each, the gradient does without them: not written and not read.)
  * cbm_b200_group_norm_grad  gx, and gw and gb [dev, channels] (NULL: not wanted).
  * cbm_b200_group_norm_workspace  bytes of workspace [dev] of either (`gradient` 0 or 1); n_samples negative: without ptr. */
 #define CBM_B200_ACT_NONE 0
@@ -404,8 +405,8 @@ int cbm_b200_group_norm(const void* x, int64_t ldx, int32_t type, int64_t n_rows
                         float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
 int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* gy, int64_t ldgy, int32_t type, int64_t n_rows,
                              int32_t channels, int32_t groups, const int64_t* ptr, int64_t n_samples, int64_t rows_each,
-                             const void* weight, const void* bias, int32_t wide_params, int32_t activation, float* mean,
-                             float* rstd, void* gx, int64_t ldgx, float* gw, float* gb, void* workspace,
+                             const void* weight, const void* bias, int32_t wide_params, float eps, int32_t activation,
+                             float* mean, float* rstd, void* gx, int64_t ldgx, float* gw, float* gb, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
 /* cbm_b200_orthogonalise     out = U orthogonalised: X = U / (|U| + eps), then `steps` times A = X X^T,
