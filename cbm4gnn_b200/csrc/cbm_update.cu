@@ -14,7 +14,8 @@
 // Work: m (m + 1) n + m^2 (m + 1) + 2 m^2 n a step, as A and A A are symmetric: only tiles that reach the upper triangle are computed,
 // and the other half is written with them.
 //
-// One kernel, three kinds of products.  A block holds a tile of 128 x BN: one warp fetches both operands' terms by TMA (64 x 64
+// One kernel, three kinds of products.  A block holds a tile of 128 x 64, or a pair of blocks on two SMs one of 256 x 128, of which each
+// fetches half of both operands: one warp fetches the operands' terms by TMA (64 x 64
 // boxes, 128-byte swizzled), one issues the MMAs, eight add up and write the result, split again, with the term that is added to it.
 // X is the second operand of X X^T with the contraction along its rows, and of B X with the contraction across them: the same boxes of
 // memory, described to the tensor cores as K-major or MN-major, so that no turned copy exists.
@@ -46,20 +47,45 @@ struct Matrix {
     float* out;      // result, where there are no weights
     int64_t ldg, ldm, ldw, ldout, next_g, next_out;
     float lr, keep;
+
+    // Up to eight values of a row of the result, 2^12 times what they are.
+    __device__ __forceinline__ void write(int64_t matrix, int row, int col, int count, const float (&v)[8]) const {
+        float* to = w ? w + row * ldw + col : out + matrix * next_out + row * ldout + col;
+        if (count == 8 && (reinterpret_cast<u64>(to) & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                float4 r = make_float4(v[i] * UNSCALE, v[i + 1] * UNSCALE, v[i + 2] * UNSCALE, v[i + 3] * UNSCALE);
+                float4* at = reinterpret_cast<float4*>(to + i);
+                if (w) {
+                    const float4 was = *at;
+                    r = make_float4(keep * was.x - lr * r.x, keep * was.y - lr * r.y, keep * was.z - lr * r.z, keep * was.w - lr * r.w);
+                }
+                *at = r;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < count) to[i] = w ? keep * to[i] - lr * (v[i] * UNSCALE) : v[i] * UNSCALE;
+        }
+    }
 };
 
 // Matrices of one shape: a stack, or one weight of a list.
-struct Job {
-    CUtensorMap x[2], a, b;    // [batch][2 terms][rows][columns], boxes of 64 x 64
+struct Shape {
     __half *px[2], *pa, *pb;
     double* parts;             // [batch][PARTS]
     Matrix of;
     int m, n, ldx, lda, turned, batch;
     int tiles_sym, tiles_all;  // of one matrix: that reach the upper triangle of A, of X
 };
+// [batch][2 terms][rows][columns]; boxes of both terms of 64 columns and 128 rows, for the first operand, or 64, for the second.
+struct Maps {
+    CUtensorMap first_x[2], first_a, first_b, second_x[2], second_a;
+};
 
 struct Jobs {
-    Job job[MAX_JOBS];
+    Maps map[MAX_JOBS];
+    Shape job[MAX_JOBS];
     int count;
     float momentum, eps;
     int nesterov;
@@ -69,7 +95,7 @@ struct Jobs {
 enum Kind { GRAM, SQUARE, APPLY };
 
 // ---- start ----------------------------------------------------------------------------------------
-__device__ __forceinline__ float update_at(const Jobs& p, const Job& q, int64_t b, int i, int j) {
+__device__ __forceinline__ float update_at(const Jobs& p, const Shape& q, int64_t b, int i, int j) {
     const float g = q.of.g[b * q.of.next_g + i * q.of.ldg + j];
     if (!q.of.m) return g;
     const float m = __ldcg(&q.of.m[i * q.of.ldm + j]);  // already this step's
@@ -81,7 +107,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ J
     cbm::wait_before();
     int j = 0, b = blockIdx.y;
     while (b >= p.job[j].batch) b -= p.job[j++].batch;
-    const Job& q = p.job[j];
+    const Shape& q = p.job[j];
     const int rows = q.turned ? q.n : q.m, cols = q.turned ? q.m : q.n;
     double s = 0.0;
     for (int i = blockIdx.x; i < rows; i += PARTS)
@@ -115,7 +141,7 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ 
     cbm::wait_before();
     int j = 0, b = blockIdx.y;
     while (b >= p.job[j].batch) b -= p.job[j++].batch;
-    const Job& q = p.job[j];
+    const Shape& q = p.job[j];
     const int across = (q.n + 31) / 32, tiles = across * ((q.m + 31) / 32), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s = 0.0;
     for (int i = 0; i < PARTS; i += 32) s += q.parts[b * PARTS + i + lane];
@@ -145,166 +171,389 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ 
 }
 
 // ---- products -------------------------------------------------------------------------------------
-template <int BN>
-struct Shape {
-    static constexpr int STAGES = BN == 64 ? 4 : 3;
-    static constexpr int A_BYTES = 4 * BOX_BYTES;             // 2 terms of 128 x 64
-    static constexpr int B_TERM = BN / 64 * BOX_BYTES;
+// SINGLE: a block to a tile.  PAIR: two blocks on neighbouring SMs to a tile, whose MMAs the first one issues for both; a block of 128 x
+// 128 would have to fetch 64 KB for 768 cycles of MMAs, 85 bytes a cycle, of which L2 gives half.  CLUSTER: everything for one
+// matrix by eight blocks, whose products follow one another without a launch between them.
+enum Mode { SINGLE, PAIR, CLUSTER };
+
+template <Mode MODE>
+struct Sizes {
+    static constexpr int BN = MODE == PAIR ? 128 : 64;        // columns of a tile
+    static constexpr int ROWS = MODE == PAIR ? 256 : 128;     // rows of a tile
+    static constexpr int STAGES = 4;
+    static constexpr int A_BYTES = 4 * BOX_BYTES;             // 2 terms of 128 x 64, of this block
+    static constexpr int B_TERM = BOX_BYTES;                  // 64 x 64
     static constexpr int STAGE = A_BYTES + 2 * B_TERM;
-    static constexpr int SMEM = STAGES * STAGE + 1024;
-    static constexpr int ACCS = 4;                             // accumulators of BN columns
+    static constexpr int TURN = 32 * 32 * 4;                  // a warp's block of 32 x 32 on its way out
+    static constexpr int SMEM = STAGES * STAGE + 8 * TURN + 1024;
+    static constexpr int ACC_COLS = 2 * BN;                   // of an accumulator, see mma_chunk
+    static constexpr int ACCS = TMEM_COLS / ACC_COLS;
 };
 
-// D[128, N] (+)= A[128, 16] B[16, N], both in shared memory.
-__device__ __forceinline__ void mma_ss(u32 d, u64 a, u64 b, u32 idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((u32)add)
-        : "memory");
+// A chunk of 64 of the contraction: with the second operand's terms h and l behind one another as one operand of twice the columns,
+// A_h [B_h | B_l] is one MMA a step, and A_l B_h the other, added to the columns from 64 on.  (So A_h is read once for two products: an
+// MMA's operands come out of shared memory at about 64 bytes a cycle, and a tile is too narrow to hide that: 256 x 128 3 x 96 cycles a step,
+// 128 + 96 so.  That bound, not L2, is also why single blocks have tiles of 64 columns.)  A block's half of the columns has its own 128:
+// h h, then h l and l h; in the second block of a pair l h comes to h h instead, which makes no difference to the sum of both.
+// Issued as one, by one elected thread: one by one, with an election and descriptors for each, twelve MMAs took 1 440 cycles.
+template <bool TWO>
+__device__ __forceinline__ void mma_chunk(u32 d, u64 ah, u64 al, u64 b, u64 next_b, u32 both, u32 one) {
+#define CBM_MMA(D, A, B, I, ADD) "@e tcgen05.mma.cta_group::" CBM_GROUP ".kind::f16 [" D "], " A ", " B ", " I ", " ADD ";\n\t"
+#define CBM_CHUNK                                                                                                              \
+    "{\n\t.reg .pred e, no, yes;\n\t.reg .b64 ah1, ah2, ah3, al1, al2, al3, b1, b2, b3;\n\t.reg .b32 d1;\n\t"                       \
+    "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 no, 0, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\tadd.u32 d1, %0, 64;\n\t"                    \
+    "add.s64 ah1, %1, 2;\n\tadd.s64 ah2, %1, 4;\n\tadd.s64 ah3, %1, 6;\n\t"                                                      \
+    "add.s64 al1, %2, 2;\n\tadd.s64 al2, %2, 4;\n\tadd.s64 al3, %2, 6;\n\t"                                                      \
+    "add.s64 b1, %3, %4;\n\tadd.s64 b2, b1, %4;\n\tadd.s64 b3, b2, %4;\n\t"                                                      \
+    CBM_MMA("%0", "%1", "%3", "%5", "no") CBM_MMA("d1", "%2", "%3", "%6", "yes") CBM_MMA("d1", "al1", "b1", "%6", "yes")       \
+    CBM_MMA("d1", "al2", "b2", "%6", "yes") CBM_MMA("d1", "al3", "b3", "%6", "yes") CBM_MMA("%0", "ah1", "b1", "%5", "yes")    \
+    CBM_MMA("%0", "ah2", "b2", "%5", "yes") CBM_MMA("%0", "ah3", "b3", "%5", "yes") "}"
+    if constexpr (TWO) {
+#define CBM_GROUP "2"
+        asm volatile(CBM_CHUNK ::"r"(d), "l"(ah), "l"(al), "l"(b), "l"(next_b), "r"(both), "r"(one) : "memory");
+#undef CBM_GROUP
+    } else {
+#define CBM_GROUP "1"
+        asm volatile(CBM_CHUNK ::"r"(d), "l"(ah), "l"(al), "l"(b), "l"(next_b), "r"(both), "r"(one) : "memory");
+#undef CBM_GROUP
+    }
+#undef CBM_CHUNK
+#undef CBM_MMA
 }
-// fp32 accumulator, fp16 operands, M = 128; bit 16: the second operand is MN-major.
-__host__ __device__ constexpr u32 idesc_half(u32 n, bool mn_major) { return (1u << 4) | ((u32)mn_major << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
+// fp32 accumulator, fp16 operands; bit 16: the second operand is MN-major.
+__host__ __device__ constexpr u32 idesc_half(u32 m, u32 n, bool mn_major) { return (1u << 4) | ((u32)mn_major << 16) | ((n >> 3) << 17) | ((m >> 4) << 24); }
 // MN-major operand of 64-wide, 128-byte swizzled blocks: 8 steps of the contraction are 1024 bytes, the next 64 columns a box further on.
 __device__ __forceinline__ u64 desc_mn(u32 addr) {
     return (u64)((addr & 0x3ffff) >> 4) | ((u64)(BOX_BYTES >> 4) << 16) | ((u64)(1024 >> 4) << 32) | ((u64)1 << 46) | ((u64)2 << 61);
 }
 
-__device__ __forceinline__ void box_in(u32 to, const CUtensorMap* map, int col, int row, int term, int matrix, u32 bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
-                 "l"(map), "r"(col), "r"(row), "r"(term), "r"(matrix), "r"(bar)
+__device__ __forceinline__ void ld32(float (&r)[32], u32 at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
+          "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
+          "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]),
+          "=f"(r[31])
+        : "r"(at));
+}
+
+// `bar` may be the other block's of a pair.  (By an elected thread of a warp that stays together, see mma; and one fetch for both terms
+// of all rows: issued one by one from a branch for lane 0, the 64 x 64 boxes took 190 cycles each, more than the MMAs waiting for them.)
+template <bool TWO>
+__device__ __forceinline__ void box_in(u32 to, const CUtensorMap* map, int col, int row, int matrix, u32 bar) {
+    if constexpr (TWO)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, 0, %4}], [%5];\n\t}" ::"r"(to),
+            "l"(map), "r"(col), "r"(row), "r"(matrix), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, 0, %4}], [%5];\n\t}" ::"r"(to),
+            "l"(map), "r"(col), "r"(row), "r"(matrix), "r"(bar)
+            : "memory");
+}
+__device__ __forceinline__ void expect(u32 bar, u32 bytes) {
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
 
+// ---- a pair of blocks -----------------------------------------------------------------------------
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// The first block's address of what lies at `local` in this one.
+__device__ __forceinline__ u32 in_first(u32 local) {
+    u32 r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(local));
+    return r;
+}
+__device__ __forceinline__ void arrive_in_first(u32 mapped) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
+}
+// In both blocks, once the MMAs issued so far are done.
+__device__ __forceinline__ void commit_both(u32 bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void pair_alloc(u32 where) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void pair_free(u32 base) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(TMEM_COLS));
+}
 struct Where {
-    int job, matrix, row, col;  // tile: rows from 128 row, columns from BN col
+    int job, matrix, row, col;  // tile: rows from ROWS row, columns from BN col
 };
-// The tile with running number t of a kind of product.
-template <int BN>
-__device__ __forceinline__ Where tile_of(const Jobs& p, Kind kind, int t) {
+// Tile t of a matrix.
+template <int ROWS, int BN>
+__device__ __forceinline__ void place(const Shape& q, Kind kind, int t, Where& w) {
+    if (kind == APPLY) {
+        // down the columns first: neighbouring blocks share X's columns, and B is small
+        const int down = (q.m + ROWS - 1) / ROWS;
+        if (down == 1) w.col = t, w.row = 0;  // (a division costs a small product a tenth of its time)
+        else if (down == 2) w.col = t >> 1, w.row = t & 1;
+        else w.col = t / down, w.row = t - w.col * down;
+        return;
+    }
+    const int across = (q.m + BN - 1) / BN;
+    w.row = 0;
+    for (int left = across; t >= left; left = across - w.row * (ROWS / BN)) t -= left, ++w.row;
+    w.col = w.row * (ROWS / BN) + t;
+}
+// The tile with running number t of a kind of product, over all matrices.
+template <int ROWS, int BN>
+__device__ __forceinline__ Where tile_of(const Shape* jobs, Kind kind, int t) {
     Where w{0, 0, 0, 0};
     for (;; ++w.job) {
-        const Job& q = p.job[w.job];
+        const Shape& q = jobs[w.job];
         const int each = kind == APPLY ? q.tiles_all : q.tiles_sym, all = each * q.batch;
         if (t >= all) {
             t -= all;
             continue;
         }
         w.matrix = t / each;
-        t -= w.matrix * each;
-        const int across = ((kind == APPLY ? q.n : q.m) + BN - 1) / BN;
-        if (kind == APPLY) {
-            // down the columns first: neighbouring blocks share X's columns, and B is small
-            const int down = (q.m + 127) / 128;
-            w.col = t / down, w.row = t % down;
-        } else {
-            for (int left = across; t >= left; left = across - w.row * (128 / BN)) t -= left, ++w.row;
-            w.col = w.row * (128 / BN) + t;
-        }
+        place<ROWS, BN>(q, kind, t - w.matrix * each, w);
         return w;
     }
 }
 
-__device__ __forceinline__ void halves8(const __half* p, float (&v)[8], float f) {
-    const uint4 w = __ldcg(reinterpret_cast<const uint4*>(p));
-    const u32 q[4] = {w.x, w.y, w.z, w.w};
+// Two fp16 terms of eight values.
+struct Terms {
+    uint4 h, l;
+    __device__ __forceinline__ void load(const __half* p, int64_t plane) {
+        h = __ldcg(reinterpret_cast<const uint4*>(p));
+        l = __ldcg(reinterpret_cast<const uint4*>(p + plane));
+    }
+    __device__ __forceinline__ void store(__half* p, int64_t plane) const {
+        *reinterpret_cast<uint4*>(p) = h;
+        *reinterpret_cast<uint4*>(p + plane) = l;
+    }
+    __device__ __forceinline__ void set(int i, u32 a, u32 b) {
+        (i == 0 ? h.x : i == 1 ? h.y : i == 2 ? h.z : h.w) = a;
+        (i == 0 ? l.x : i == 1 ? l.y : i == 2 ? l.z : l.w) = b;
+    }
+    // Both terms of value j in one word, the first below; and back.
+    __device__ __forceinline__ u32 word(int j) const {
+        const u32 a = j < 2 ? h.x : j < 4 ? h.y : j < 6 ? h.z : h.w, b = j < 2 ? l.x : j < 4 ? l.y : j < 6 ? l.z : l.w;
+        return __byte_perm(a, b, j & 1 ? 0x7632 : 0x5410);
+    }
+    __device__ __forceinline__ void pair(int i, u32 first, u32 second) {
+        set(i, __byte_perm(first, second, 0x5410), __byte_perm(first, second, 0x7632));
+    }
+    // v += f * these
+    __device__ __forceinline__ void add_to(float (&v)[8], float f) const {
+        const u32 x[4] = {h.x, h.y, h.z, h.w}, y[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 s = __half22float2(reinterpret_cast<const __half2&>(x[i])), t = __half22float2(reinterpret_cast<const __half2&>(y[i]));
+            v[2 * i] += f * s.x + f * t.x;
+            v[2 * i + 1] += f * s.y + f * t.y;
+        }
+    }
+};
+// The two terms of eight values.  (Two values a conversion: one by one they are converted at a quarter of the rate.)
+__device__ __forceinline__ Terms terms_of(const float (&v)[8]) {
+    Terms t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&q[i]));
-        v[2 * i] += f * t.x, v[2 * i + 1] += f * t.y;
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+        t.set(i, reinterpret_cast<const u32&>(h), reinterpret_cast<const u32&>(l));
     }
+    return t;
 }
 
-template <int BN>
-__global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const Kind kind, const int from, const int tiles,
-                                                                  const bool last) {
-    using S = Shape<BN>;
+// What a cluster's blocks wrote is seen by all of them, their TMA fetches included.
+__device__ __forceinline__ void cluster_turn(bool wrote, bool fetches) {
+    if (wrote) asm volatile("fence.proxy.async;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (fetches) asm volatile("fence.proxy.async;" ::: "memory");
+}
+
+// In a cluster of `blocks`, all threads: momentum, norm and X, split, of one matrix.
+__device__ __forceinline__ void start_in_cluster(const Jobs& p, const Shape& q, int b, int rank, int blocks, double* s_part) {
+    const int rows = q.turned ? q.n : q.m, cols = q.turned ? q.m : q.n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double s = 0.0;
+    for (int i = rank * (TILE_THREADS / 32) + warp; i < rows; i += blocks * (TILE_THREADS / 32))
+        for (int c = lane; c < cols; c += 32) {
+            if (q.of.m) {
+                float* m = &q.of.m[i * q.of.ldm + c];
+                *m = p.momentum * *m + q.of.g[i * q.of.ldg + c];
+            }
+            const double u = update_at(p, q, b, i, c);
+            s += u * u;
+        }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) s_part[warp] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < TILE_THREADS / 32; ++i) s += s_part[i];
+        __stcg(&q.parts[b * PARTS + rank], s);
+    }
+    cluster_turn(false, false);
+    s = 0.0;
+    for (int i = 0; i < blocks; ++i) s += __ldcg(&q.parts[b * PARTS + i]);
+    const double scale = (double)SCALE / (sqrt(s) + (double)p.eps);
+    const int64_t plane = (int64_t)q.m * q.ldx;
+    __half* x = q.px[0] + 2 * b * plane;
+    for (int i = rank * (TILE_THREADS / 32) + warp; i < rows; i += blocks * (TILE_THREADS / 32))
+        for (int c = lane; c < cols; c += 32) {
+            __half h, l;
+            split((float)((double)update_at(p, q, b, i, c) * scale), h, l);
+            const int64_t at = q.turned ? (int64_t)c * q.ldx + i : (int64_t)i * q.ldx + c;
+            x[at] = h;
+            x[at + plane] = l;
+        }
+    cluster_turn(true, true);
+}
+
+// One kind of product over the tiles of all matrices; or, with CLUSTER, all products of one.
+template <Mode MODE>
+__global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const Kind only, const int first_from,
+                                                                  const int all_tiles, const bool only_last, const int steps) {
+    using S = Sizes<MODE>;
+    constexpr int BN = S::BN;
+    constexpr bool TWO = MODE == PAIR;
     extern __shared__ unsigned char smem_raw[];
     __shared__ u64 s_bar[2 * S::STAGES + 2 * S::ACCS + 1];
     __shared__ u32 s_tmem;
     __shared__ int s_gave_up;
+    __shared__ double s_norm[MODE == CLUSTER ? TILE_THREADS / 32 : 1];
+    // (at an index that is not known beforehand, parameters are read from the constant bank at hundreds of cycles a time)
+    __shared__ Shape s_jobs[MAX_JOBS];
     const u32 smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const u32 full = smem_u32(s_bar), empty = full + 8 * S::STAGES, acc_full = empty + 8 * S::STAGES, acc_empty = acc_full + 8 * S::ACCS,
               drained = acc_empty + 8 * S::ACCS;
-    if (warp == ISSUER) tmem_alloc(smem_u32(&s_tmem));
+    if (warp == ISSUER) {
+        if constexpr (TWO) pair_alloc(smem_u32(&s_tmem));
+        else tmem_alloc(smem_u32(&s_tmem));
+    }
+    for (int i = threadIdx.x; i < p.count * (int)(sizeof(Shape) / 4); i += TILE_THREADS)
+        reinterpret_cast<u32*>(s_jobs)[i] = reinterpret_cast<const u32*>(p.job)[i];
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; ++s) bar_init(full + 8 * s, 1), bar_init(empty + 8 * s, 1);
-        for (int s = 0; s < S::ACCS; ++s) bar_init(acc_full + 8 * s, 1), bar_init(acc_empty + 8 * s, 8);
+        for (int s = 0; s < S::ACCS; ++s) bar_init(acc_full + 8 * s, 1), bar_init(acc_empty + 8 * s, TWO ? 16 : 8);
         bar_init(drained, 1);
         s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     fence_before();
     __syncthreads();
+    if constexpr (TWO) cluster_barrier();  // the other block's barriers and tensor memory are there
     fence_after();
     const u32 tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     volatile int* gave_up = &s_gave_up;
     cbm::wait_before();
+    int rank = blockIdx.x, stride = gridDim.x, side = 0;  // (side: which block of a pair)
+    if constexpr (TWO) {
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(side));
+        rank >>= 1, stride >>= 1;
+    }
+    auto wait = [&](u32 bar, u32 parity) { return warp_wait(bar, parity, gave_up, p.timeout); };
+    Where one{0, 0, 0, 0};
+    if constexpr (MODE == CLUSTER) {
+        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(stride));
+        one.matrix = blockIdx.x / stride;
+        while (one.matrix >= s_jobs[one.job].batch) one.matrix -= s_jobs[one.job++].batch;
+        start_in_cluster(p, s_jobs[one.job], one.matrix, rank, stride, s_norm);
+    }
+    // f(kind, the buffer X is in, whether it is the last product): in a cluster all blocks go from one product to the next together,
+    // those that have given up, too.
+    auto each_product = [&](auto&& f) {
+        if constexpr (MODE != CLUSTER) {
+            f(only, first_from, only_last);
+        } else {
+            for (int k = 0; k < steps; ++k)
+                for (int kind = GRAM; kind <= APPLY; ++kind) {
+                    f((Kind)kind, k & 1, k + 1 == steps);
+                    if (kind != APPLY || k + 1 < steps) cluster_turn(warp < PRODUCER, warp == PRODUCER);
+                }
+        }
+    };
+    auto tiles_of = [&](Kind kind) { return MODE != CLUSTER ? all_tiles : kind == APPLY ? s_jobs[one.job].tiles_all : s_jobs[one.job].tiles_sym; };
+    auto find = [&](Kind kind, int t) {
+        if constexpr (MODE != CLUSTER) return tile_of<S::ROWS, BN>(s_jobs, kind, t);
+        Where w = one;
+        place<S::ROWS, BN>(s_jobs[w.job], kind, t, w);
+        return w;
+    };
 
     if (warp == PRODUCER) {
+        const u32 first_full = TWO ? in_first(full) : full;
         u32 it = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const Where w = tile_of<BN>(p, kind, t);
-            const Job& q = p.job[w.job];
-            const int depth = kind == GRAM ? q.n : q.m, width = kind == APPLY ? q.n : q.m;
-            const CUtensorMap *ma = kind == GRAM ? &q.x[from] : kind == SQUARE ? &q.a : &q.b, *mb = kind == SQUARE ? &q.a : &q.x[from];
-            // boxes that lie past the matrix are left out: their rows and columns of the tile are not written
-            const int boxes_a = q.m - 128 * w.row > 64 ? 2 : 1, boxes_b = min((width - BN * w.col + 63) / 64, BN / 64);
+        each_product([&](Kind kind, int from, bool) {
+          for (int t = rank; t < tiles_of(kind) && ok; t += stride) {
+            const Where w = find(kind, t);
+            const Shape& q = s_jobs[w.job];
+            const int depth = kind == GRAM ? q.n : q.m;
+            const Maps& maps = p.map[w.job];
+            const CUtensorMap* ma = kind == GRAM ? &maps.first_x[from] : kind == SQUARE ? &maps.first_a : &maps.first_b;
+            const CUtensorMap* mb = kind == SQUARE ? &maps.second_a : &maps.second_x[from];
+            const int row0 = S::ROWS * w.row + 128 * side, col0 = BN * w.col + 64 * side;
             for (int k = 0; k < depth; k += 64, ++it) {
-                const u32 slot = it % S::STAGES, use = it / S::STAGES, bar = full + 8 * slot, at = smem + slot * S::STAGE;
-                if (use > 0 && !(ok = warp_wait(empty + 8 * slot, (use + 1) & 1, gave_up, p.timeout))) break;
-                if (lane == 0) {
-                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * (boxes_a + boxes_b) * BOX_BYTES) : "memory");
-                    for (int term = 0; term < 2; ++term) {
-                        for (int i = 0; i < boxes_a; ++i) box_in(at + (2 * term + i) * BOX_BYTES, ma, k, 128 * w.row + 64 * i, term, w.matrix, bar);
-                        for (int i = 0; i < boxes_b; ++i) {
-                            const u32 to = at + S::A_BYTES + term * S::B_TERM + i * BOX_BYTES;
-                            if (kind == APPLY) box_in(to, mb, BN * w.col + 64 * i, k, term, w.matrix, bar);
-                            else box_in(to, mb, k, BN * w.col + 64 * i, term, w.matrix, bar);
-                        }
-                    }
-                }
+                const u32 slot = it % S::STAGES, use = it / S::STAGES, at = smem + slot * S::STAGE;
+                if (use > 0 && !(ok = wait(empty + 8 * slot, (use + 1) & 1))) break;
+                // (what lies past the matrix comes as zeros; the first block of a pair answers for both)
+                if (side == 0) expect(full + 8 * slot, TWO ? 2 * S::STAGE : S::STAGE);
+                box_in<TWO>(at, ma, k, row0, w.matrix, first_full + 8 * slot);
+                if (kind == APPLY) box_in<TWO>(at + S::A_BYTES, mb, col0, k, w.matrix, first_full + 8 * slot);
+                else box_in<TWO>(at + S::A_BYTES, mb, k, col0, w.matrix, first_full + 8 * slot);
                 __syncwarp();
             }
-        }
+          }
+        });
         // What was fetched has arrived before the block leaves, also where others have given up.
-        for (u32 back = 1; back <= (u32)S::STAGES && back <= it; ++back) {
+        // (The second block of a pair is told by the first, with the barrier at the end.)
+        for (u32 back = 1; side == 0 && back <= (u32)S::STAGES && back <= it; ++back) {
             const u32 i = it - back;
             for (u32 spins = 0; spins < (1u << 22) && !bar_poll(full + 8 * (i % S::STAGES), (i / S::STAGES) & 1); ++spins) {
             }
         }
         __syncwarp();
     } else if (warp == ISSUER) {
-        const u32 idesc = idesc_half(BN, kind == APPLY);
         u32 it = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            const Where w = tile_of<BN>(p, kind, t);
-            const Job& q = p.job[w.job];
+        each_product([&](Kind kind, int, bool) {
+          const u32 both = idesc_half(S::ROWS, 2 * BN, kind == APPLY), one_term = idesc_half(S::ROWS, BN, kind == APPLY);
+          for (int t = rank; t < tiles_of(kind) && ok && side == 0; t += stride) {
+            const Where w = find(kind, t);
+            const Shape& q = s_jobs[w.job];
             const int depth = kind == GRAM ? q.n : q.m;
             for (int k = 0; k < depth; k += 64, ++it) {
                 const u32 slot = it % S::STAGES, use = it / S::STAGES, at = smem + slot * S::STAGE;
-                const u32 as = it % S::ACCS, acc_use = it / S::ACCS, d = tmem + as * BN;
-                if (acc_use > 0 && !(ok = warp_wait(acc_empty + 8 * as, (acc_use + 1) & 1, gave_up, p.timeout))) break;
-                if (!(ok = warp_wait(full + 8 * slot, use & 1, gave_up, p.timeout))) break;
-                const int steps = min(4, (depth - k + 15) / 16);
-                bool add = false;
-#pragma unroll
-                for (int pass = 0; pass < 3; ++pass) {  // l h, h l, h h
-                    const u32 a = at + (pass == 0 ? 2 * BOX_BYTES : 0), b = at + S::A_BYTES + (pass == 1 ? S::B_TERM : 0);
-                    for (int s = 0; s < steps; ++s) {
-                        mma_ss(d, desc_of(a + 32 * s), kind == APPLY ? desc_mn(b + 2048 * s) : desc_of(b + 32 * s), idesc, add);
-                        add = true;
-                    }
+                const u32 as = it % S::ACCS, acc_use = it / S::ACCS, d = tmem + as * S::ACC_COLS;
+                if (acc_use > 0 && !(ok = wait(acc_empty + 8 * as, (acc_use + 1) & 1))) break;
+                if (!(ok = wait(full + 8 * slot, use & 1))) break;
+                const u64 ah = desc_of(at), al = desc_of(at + 2 * BOX_BYTES);
+                // (what lies past the last column of the contraction has been fetched as zeros)
+                if (kind == APPLY) mma_chunk<TWO>(d, ah, al, desc_mn(at + S::A_BYTES), 2048 >> 4, both, one_term);
+                else mma_chunk<TWO>(d, ah, al, desc_of(at + S::A_BYTES), 32 >> 4, both, one_term);
+                if constexpr (TWO) {
+                    commit_both(empty + 8 * slot);
+                    commit_both(acc_full + 8 * as);
+                } else {
+                    commit(empty + 8 * slot);
+                    commit(acc_full + 8 * as);
                 }
-                commit(empty + 8 * slot);
-                commit(acc_full + 8 * as);
             }
-        }
+          }
+        });
         if (!ok) {  // the MMAs under way end before the block frees its tensor memory
-            commit(drained);
+            if constexpr (TWO) commit_both(drained);
+            else commit(drained);
             for (u32 spins = 0; spins < (1u << 20) && !bar_poll(drained, 0); ++spins) {
             }
             __syncwarp();
@@ -312,91 +561,137 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
     } else {
         const int quarter = warp & 3, half = warp >> 2;
         constexpr int EACH = BN / 2;  // columns of this warp
+        float4* turn = reinterpret_cast<float4*>(smem_raw + (smem - smem_u32(smem_raw)) + S::STAGES * S::STAGE) + warp * (S::TURN / 16);
         u32 it = 0;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-            const Where w = tile_of<BN>(p, kind, t);
-            const Job& q = p.job[w.job];
+        bool ok = true;
+        each_product([&](Kind kind, int from, bool last) {
+          for (int t = rank; t < tiles_of(kind) && ok; t += stride) {
+            const Where w = find(kind, t);
+            const Shape& q = s_jobs[w.job];
             const int depth = kind == GRAM ? q.n : q.m, width = kind == APPLY ? q.n : q.m, ld = kind == APPLY ? q.ldx : q.lda;
             float sum[EACH];
 #pragma unroll
             for (int i = 0; i < EACH; ++i) sum[i] = 0.f;
-            bool ok = true;
             for (int k = 0; k < depth; k += 64, ++it) {
                 const u32 as = it % S::ACCS, use = it / S::ACCS;
-                if (!(ok = warp_wait(acc_full + 8 * as, use & 1, gave_up, p.timeout))) break;
-                const u32 at = tmem + as * BN + half * EACH + ((u32)(quarter * 32) << 16);
+                if (!(ok = wait(acc_full + 8 * as, use & 1))) break;
+                const u32 at = tmem + as * S::ACC_COLS + half * (TWO ? 128 : EACH) + ((u32)(quarter * 32) << 16);
 #pragma unroll
-                for (int c = 0; c < EACH; c += 16) {
-                    float r[16];
-                    asm volatile(
-                        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
-                          "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
-                        : "r"(at + c));
+                for (int c = 0; c < EACH; c += 32) {
+                    float r[2][32];
+                    ld32(r[0], at + c);
+                    ld32(r[1], at + 64 + c);
                     wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(r[i]));  // not before the wait
+                    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(r[0][i]), "+f"(r[1][i]));  // not before the wait
+                    if (c + 32 == EACH) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (TWO) arrive_in_first(in_first(acc_empty + 8 * as));
+                            else bar_arrive(acc_empty + 8 * as);
+                        }
+                    }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) add2(sum[c + i], sum[c + i + 1], r[i], r[i + 1]);
+                    for (int i = 0; i < 32; i += 2) {
+                        add2(r[0][i], r[0][i + 1], r[1][i], r[1][i + 1]);
+                        add2(sum[c + i], sum[c + i + 1], r[0][i], r[0][i + 1]);
+                    }
                 }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(acc_empty + 8 * as);
             }
             if (!ok) break;
-            const int row = 128 * w.row + 32 * quarter + lane, col0 = BN * w.col + half * EACH;
-            const int64_t plane = (int64_t)q.m * ld, matrix = 2 * w.matrix * plane;
-            __half* to = (kind == GRAM ? q.pa : kind == SQUARE ? q.pb : q.px[from ^ 1]) + matrix + (int64_t)row * ld;
-            const __half* more = (kind == SQUARE ? q.pa : q.px[from]) + matrix + (int64_t)row * ld;
+            const int m = q.m;
+            const int64_t plane = (int64_t)m * ld, matrix = 2 * w.matrix * plane;
+            __half* to = (kind == GRAM ? q.pa : kind == SQUARE ? q.pb : q.px[from ^ 1]) + matrix;
+            const __half* more = (kind == SQUARE ? q.pa : q.px[from]) + matrix;
+            const float factor = kind == SQUARE ? QUINTIC_C * UNSCALE : UNSCALE, more_factor = kind == SQUARE ? QUINTIC_B : QUINTIC_A;
+            const bool result = kind == APPLY && last, turned = result && q.turned;
+            const Matrix of = q.of;
+            // 32 x 32 values at a time: as they were summed up a lane has a row; then it has eight neighbours of a row, four times.
+            const int row0 = S::ROWS * w.row + 128 * side + 32 * quarter, row = row0 + (lane >> 2);
+            Terms add[EACH / 32][4];
+            if (kind != GRAM) {
 #pragma unroll
-            for (int c = 0; c < EACH; c += 8) {
-                const int col = col0 + c;
-                if (row >= q.m || col >= width) break;
-                if (kind != APPLY && col + 8 <= row) continue;  // below the diagonal: written by the tile above it
-                float v[8];
+                for (int block = 0; block < EACH / 32; ++block)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = sum[c + i] * (kind == SQUARE ? QUINTIC_C * UNSCALE : UNSCALE);
-                if (kind != GRAM) {
-                    const float f = kind == SQUARE ? QUINTIC_B : QUINTIC_A;
-                    halves8(more + col, v, f);
-                    halves8(more + plane + col, v, f);
-                }
-                if (kind == APPLY && last) {
-                    const Matrix& o = q.of;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (col + i >= q.n) break;
-                        const int64_t r = q.turned ? col + i : row, s = q.turned ? row : col + i;
-                        if (o.w) o.w[r * o.ldw + s] = o.keep * o.w[r * o.ldw + s] - o.lr * (v[i] * UNSCALE);
-                        else o.out[w.matrix * o.next_out + r * o.ldout + s] = v[i] * UNSCALE;
+                    for (int i = 0; i < 4; ++i) {
+                        const int col = BN * w.col + half * EACH + 32 * block + 8 * (lane & 3);
+                        if (row + 8 * i < m && col < width) add[block][i].load(more + (int64_t)(row + 8 * i) * ld + col, plane);
                     }
-                    continue;
-                }
-                __half h[8], l[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) split(v[i], h[i], l[i]);
-                if (kind == APPLY || col >= row) {  // (the row's padding may be written over)
-                    *reinterpret_cast<uint4*>(to + col) = *reinterpret_cast<const uint4*>(h);
-                    *reinterpret_cast<uint4*>(to + plane + col) = *reinterpret_cast<const uint4*>(l);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (col + i >= row) to[col + i] = h[i], to[plane + col + i] = l[i];
-                }
-                if (kind != APPLY) {
-                    __half* across = (kind == GRAM ? q.pa : q.pb) + matrix + row;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (col + i > row && col + i < q.m) across[(int64_t)(col + i) * ld] = h[i], across[plane + (int64_t)(col + i) * ld] = l[i];
-                }
             }
-            __syncwarp();
-        }
+#pragma unroll
+            for (int block = 0; block < EACH / 32; ++block) {
+                const int col0 = BN * w.col + half * EACH + 32 * block, col = col0 + 8 * (lane & 3);
+                if (row0 >= m || col0 >= width || (kind != APPLY && col0 < row0)) continue;  // (below the diagonal: written across)
+                // Four columns of a row lie together, those of row r at (column / 4) ^ swirl(r): no two lanes meet in a bank, by rows or by
+                // columns.
+                auto swirl = [](int r) { return (r & 7) ^ (r >> 3 << 1); };
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    turn[lane * 8 + (c ^ swirl(lane))] = make_float4(sum[32 * block + 4 * c], sum[32 * block + 4 * c + 1], sum[32 * block + 4 * c + 2], sum[32 * block + 4 * c + 3]);
+                __syncwarp();
+                const bool across = kind != APPLY && col0 > row0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int in_row = 8 * i + (lane >> 2);
+                    float4 &lo = turn[in_row * 8 + ((2 * (lane & 3)) ^ swirl(in_row))], &hi = turn[in_row * 8 + ((2 * (lane & 3) + 1) ^ swirl(in_row))];
+                    const float4 x = lo, y = hi;
+                    float v[8] = {factor * x.x, factor * x.y, factor * x.z, factor * x.w, factor * y.x, factor * y.y, factor * y.z, factor * y.w};
+                    const bool in = row + 8 * i < m && col < width;
+                    if (kind != GRAM && in) add[block][i].add_to(v, more_factor);
+                    if (turned) {
+                        lo = make_float4(v[0], v[1], v[2], v[3]);
+                        hi = make_float4(v[4], v[5], v[6], v[7]);
+                    } else if (result) {
+                        if (in) of.write(w.matrix, row + 8 * i, col, min(8, width - col), v);
+                    } else {
+                        const Terms t = terms_of(v);
+                        if (in) t.store(to + (int64_t)(row + 8 * i) * ld + col, plane);  // (the row's padding may be written over)
+                        if (across) {
+                            reinterpret_cast<uint4&>(lo) = make_uint4(t.word(0), t.word(1), t.word(2), t.word(3));
+                            reinterpret_cast<uint4&>(hi) = make_uint4(t.word(4), t.word(5), t.word(6), t.word(7));
+                        }
+                    }
+                }
+                __syncwarp();
+                if (across || turned) {  // the same values, turned: eight neighbours of a column
+                    const int r = row0 + 8 * (lane & 3), c = col0 + (lane >> 2);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int column = 8 * i + (lane >> 2);
+                        u32 words[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int at = 8 * (lane & 3) + j;
+                            words[j] = reinterpret_cast<const u32*>(turn)[at * 32 + (((column >> 2) ^ swirl(at)) << 2) + (column & 3)];
+                        }
+                        if (r >= m || c + 8 * i >= width) continue;
+                        if (across) {
+                            Terms t;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) t.pair(j, words[2 * j], words[2 * j + 1]);
+                            t.store(to + (int64_t)(c + 8 * i) * ld + r, plane);
+                        } else {
+                            float v[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(words[j]);
+                            of.write(w.matrix, c + 8 * i, r, min(8, m - r), v);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+          }
+        });
     }
     fence_before();
     __syncthreads();
+    if constexpr (TWO) cluster_barrier();  // nothing of the other block is under way here any more
     fence_after();
-    if (warp == ISSUER) tmem_free(tmem);
+    if (warp == ISSUER) {
+        if constexpr (TWO) pair_free(tmem);
+        else tmem_free(tmem);
+    }
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -416,12 +711,12 @@ Encode encoder() {
     return encode;
 }
 
-bool describe(CUtensorMap* map, const __half* p, int rows, int cols, int ld, int batch) {
+bool describe(CUtensorMap* map, const __half* p, int rows, int cols, int ld, int batch, int box_rows) {
     const Encode encode = encoder();
     if (!encode) return false;
     const cuuint64_t size[4] = {(cuuint64_t)cols, (cuuint64_t)rows, 2, (cuuint64_t)batch};
     const cuuint64_t pitch[3] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * rows, (cuuint64_t)ld * 4 * rows};
-    const cuuint32_t box[4] = {64, 64, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 2, 1}, step[4] = {1, 1, 1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(p), size, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -429,7 +724,7 @@ bool describe(CUtensorMap* map, const __half* p, int rows, int cols, int ld, int
 int64_t pad(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Workspace of a job, and where its arrays lie in it.
-int64_t lay_out(Job* q, int rows, int cols, int batch, unsigned char* at) {
+int64_t lay_out(Shape* q, int rows, int cols, int batch, unsigned char* at) {
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     const int ldx = (n + 7) / 8 * 8, lda = (m + 7) / 8 * 8;
     const int64_t x = pad((int64_t)4 * batch * m * ldx), a = pad((int64_t)4 * batch * m * lda), parts = pad((int64_t)8 * batch * PARTS);
@@ -442,29 +737,74 @@ int64_t lay_out(Job* q, int rows, int cols, int batch, unsigned char* at) {
     return 2 * x + 2 * a + parts;
 }
 
-int tiles_sym(int m, int bn) {
+template <Mode MODE>
+int tiles_sym(int m) {
+    using S = Sizes<MODE>;
     int t = 0;
-    for (int r = 0; r * 128 < m; ++r) t += (m + bn - 1) / bn - r * (128 / bn);
+    for (int r = 0; r * S::ROWS < m; ++r) t += (m + S::BN - 1) / S::BN - r * (S::ROWS / S::BN);
     return t;
 }
-int tiles_all(int m, int n, int bn) { return (m + 127) / 128 * ((n + bn - 1) / bn); }
+template <Mode MODE>
+int tiles_all(int m, int n) {
+    using S = Sizes<MODE>;
+    return (m + S::ROWS - 1) / S::ROWS * ((n + S::BN - 1) / S::BN);
+}
 
-template <int BN>
+template <Mode MODE>
+void launch(dim3 grid, int cluster, const cbm::Stream& on, const Jobs& p, Kind kind, int from, int tiles, bool last, int steps) {
+    cudaLaunchAttribute attrs[2] = {};
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = cluster;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(TILE_THREADS);
+    config.dynamicSmemBytes = Sizes<MODE>::SMEM;
+    config.stream = on.s;
+    config.attrs = attrs;
+    config.numAttrs = on.captured ? 1 : 2;
+    (void)cudaLaunchKernelEx(&config, product_kernel<MODE>, p, kind, from, tiles, last, steps);
+}
+
+// A launch for every product, of all matrices.
+template <Mode MODE>
 int products(const char* who, Jobs& p, int steps, const cbm::Stream& on) {
-    using S = Shape<BN>;
-    if (!allow_smem<product_kernel<BN>>(S::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
-    int sym = 0, all = 0;
+    if (!allow_smem<product_kernel<MODE>>(Sizes<MODE>::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
+    int sym = 0, all = 0, matrices = 0, blocks = 1;
     for (int i = 0; i < p.count; ++i) {
-        Job& q = p.job[i];
-        q.tiles_sym = tiles_sym(q.m, BN), q.tiles_all = tiles_all(q.m, q.n, BN);
-        sym += q.tiles_sym * q.batch, all += q.tiles_all * q.batch;
+        Shape& q = p.job[i];
+        q.tiles_sym = tiles_sym<MODE>(q.m), q.tiles_all = tiles_all<MODE>(q.m, q.n);
+        sym += q.tiles_sym * q.batch, all += q.tiles_all * q.batch, matrices += q.batch;
+        const int64_t tiles = (int64_t)((q.m + 31) / 32) * ((q.n + 31) / 32);
+        if (tiles > blocks) blocks = (int)(tiles < 2048 ? tiles : 2048);
     }
-    const int sms = sm_count();
+    cbm::launch_next(norm_kernel, dim3(PARTS, matrices), THREADS, 0, on, p);
+    cbm::launch_next(start_kernel, dim3(blocks, matrices), THREADS, 0, on, p);
+    const int cluster = MODE == PAIR ? 2 : 1, most = sm_count() / cluster;
+    const dim3 for_sym((sym < most ? sym : most) * cluster), for_all((all < most ? all : most) * cluster);
     for (int k = 0; k < steps; ++k) {
-        cbm::launch_next(product_kernel<BN>, dim3(sym < sms ? sym : sms), TILE_THREADS, S::SMEM, on, p, GRAM, k & 1, sym, false);
-        cbm::launch_next(product_kernel<BN>, dim3(sym < sms ? sym : sms), TILE_THREADS, S::SMEM, on, p, SQUARE, k & 1, sym, false);
-        cbm::launch_next(product_kernel<BN>, dim3(all < sms ? all : sms), TILE_THREADS, S::SMEM, on, p, APPLY, k & 1, all, k + 1 == steps);
+        launch<MODE>(for_sym, cluster, on, p, GRAM, k & 1, sym, false, 0);
+        launch<MODE>(for_sym, cluster, on, p, SQUARE, k & 1, sym, false, 0);
+        launch<MODE>(for_all, cluster, on, p, APPLY, k & 1, all, k + 1 == steps, 0);
     }
+    return CBM_B200_OK;
+}
+
+// One launch for everything, a cluster of blocks to a matrix.
+constexpr int CLUSTER_BLOCKS = 8, CLUSTER_TILES = 16;
+bool fits_cluster(int m, int n) { return tiles_sym<CLUSTER>(m) <= CLUSTER_BLOCKS && tiles_all<CLUSTER>(m, n) <= CLUSTER_TILES; }
+
+int clusters(const char* who, Jobs& p, int steps, const cbm::Stream& on) {
+    if (!allow_smem<product_kernel<CLUSTER>>(Sizes<CLUSTER>::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
+    int matrices = 0;
+    for (int i = 0; i < p.count; ++i) {
+        Shape& q = p.job[i];
+        q.tiles_sym = tiles_sym<CLUSTER>(q.m), q.tiles_all = tiles_all<CLUSTER>(q.m, q.n);
+        matrices += q.batch;
+    }
+    launch<CLUSTER>(dim3(matrices * CLUSTER_BLOCKS), CLUSTER_BLOCKS, on, p, GRAM, 0, 0, false, steps);
     return CBM_B200_OK;
 }
 
@@ -472,22 +812,23 @@ int run(const char* who, Jobs& p, int steps, void* stream) {
     if (int rc = check_timeout(who)) return rc;
     p.timeout = timeout_word();
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
-    int matrices = 0, blocks = 1;
-    int64_t wide = 0;
+    int64_t pairs = 0;
+    bool small = true;
     for (int i = 0; i < p.count; ++i) {
-        Job& q = p.job[i];
-        if (!describe(&q.x[0], q.px[0], q.m, q.n, q.ldx, q.batch) || !describe(&q.x[1], q.px[1], q.m, q.n, q.ldx, q.batch) ||
-            !describe(&q.a, q.pa, q.m, q.m, q.lda, q.batch) || !describe(&q.b, q.pb, q.m, q.m, q.lda, q.batch))
+        Shape& q = p.job[i];
+        Maps& map = p.map[i];
+        bool done = describe(&map.first_a, q.pa, q.m, q.m, q.lda, q.batch, 128) && describe(&map.second_a, q.pa, q.m, q.m, q.lda, q.batch, 64) &&
+                    describe(&map.first_b, q.pb, q.m, q.m, q.lda, q.batch, 128);
+        for (int k = 0; k < 2; ++k)
+            done = done && describe(&map.first_x[k], q.px[k], q.m, q.n, q.ldx, q.batch, 128) && describe(&map.second_x[k], q.px[k], q.m, q.n, q.ldx, q.batch, 64);
+        if (!done)
             return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no tensor map for its operands");
-        matrices += q.batch;
-        const int64_t tiles = (int64_t)((q.m + 31) / 32) * ((q.n + 31) / 32);
-        if (tiles > blocks) blocks = (int)(tiles < 2048 ? tiles : 2048);
-        wide += (int64_t)q.batch * tiles_sym(q.m, 128);
+        pairs += (int64_t)q.batch * tiles_sym<PAIR>(q.m);
+        small = small && fits_cluster(q.m, q.n);
     }
-    cbm::launch_next(norm_kernel, dim3(PARTS, matrices), THREADS, 0, on, p);
-    cbm::launch_next(start_kernel, dim3(blocks, matrices), THREADS, 0, on, p);
-    // Tiles of 128 columns where there are enough of them for most SMs, else of 64.
-    if (int rc = wide * 4 >= sm_count() * 3 ? products<128>(who, p, steps, on) : products<64>(who, p, steps, on)) return rc;
+    // Pairs of blocks where there are tiles of 256 x 128 for half of them at least, else single ones.
+    const int rc = small ? clusters(who, p, steps, on) : pairs * 4 >= sm_count() ? products<PAIR>(who, p, steps, on) : products<SINGLE>(who, p, steps, on);
+    if (rc) return rc;
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
@@ -537,19 +878,22 @@ extern "C" int cbm_b200_orthogonal_step(const cbm_b200_update_of* of, int32_t co
     if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need))
         return cbm::fail(CBM_B200_ERR_ARG, "orthogonal_step: workspace too small, or not at 256 bytes");
     unsigned char* at = static_cast<unsigned char*>(workspace);
-    for (int i = 0; i < count;) {
-        Jobs p{};
-        p.eps = eps, p.momentum = momentum, p.nesterov = nesterov;
-        for (; i < count && p.count < MAX_JOBS; ++i) {
-            const cbm_b200_update_of& u = of[i];
-            if (u.rows == 0 || u.cols == 0) continue;
-            Job& q = p.job[p.count++];
-            at += lay_out(&q, u.rows, u.cols, 1, at);
-            const double tall = u.rows > u.cols ? std::sqrt((double)u.rows / u.cols) : 1.0;
-            q.of = Matrix{u.g, u.m, u.w, nullptr, u.ldg, u.ldm, u.ldw, 0, 0, 0, (float)(lr * tall), (float)(1.0 - (double)lr * weight_decay)};
+    // Those that a cluster of blocks does by itself, and the others.
+    for (int small = 1; small >= 0; --small)
+        for (int i = 0; i < count;) {
+            Jobs p{};
+            p.eps = eps, p.momentum = momentum, p.nesterov = nesterov;
+            for (; i < count && p.count < MAX_JOBS; ++i) {
+                const cbm_b200_update_of& u = of[i];
+                const int m = u.rows < u.cols ? u.rows : u.cols, n = u.rows < u.cols ? u.cols : u.rows;
+                if (m == 0 || fits_cluster(m, n) != (small != 0)) continue;
+                Shape& q = p.job[p.count++];
+                at += lay_out(&q, u.rows, u.cols, 1, at);
+                const double tall = u.rows > u.cols ? std::sqrt((double)u.rows / u.cols) : 1.0;
+                q.of = Matrix{u.g, u.m, u.w, nullptr, u.ldg, u.ldm, u.ldw, 0, 0, 0, (float)(lr * tall), (float)(1.0 - (double)lr * weight_decay)};
+            }
+            if (p.count)
+                if (int rc = run("orthogonal_step", p, steps, stream)) return rc;
         }
-        if (p.count)
-            if (int rc = run("orthogonal_step", p, steps, stream)) return rc;
-    }
     return CBM_B200_OK;
 }
