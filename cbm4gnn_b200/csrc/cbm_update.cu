@@ -90,6 +90,7 @@ struct Jobs {
     float momentum, eps;
     int nesterov;
     int* timeout;
+    u32* arrived;              // of the products' blocks, zeroed by the first kernel
 };
 
 enum Kind { GRAM, SQUARE, APPLY };
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ J
     if (threadIdx.x == 0) {
         for (int i = 1; i < THREADS / 32; ++i) s += part[i];
         q.parts[b * PARTS + blockIdx.x] = s;
+        if (blockIdx.x == 0 && blockIdx.y == 0) *p.arrived = 0;
     }
 }
 
@@ -171,10 +173,8 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ 
 }
 
 // ---- products -------------------------------------------------------------------------------------
-// SINGLE: a block to a tile.  PAIR: two blocks on neighbouring SMs to a tile, whose MMAs the first one issues for both; a block of 128 x
-// 128 would have to fetch 64 KB for 768 cycles of MMAs, 85 bytes a cycle, of which L2 gives half.  CLUSTER: everything for one
-// matrix by eight blocks, whose products follow one another without a launch between them.
-enum Mode { SINGLE, PAIR, CLUSTER };
+// SINGLE: a block to a tile.  PAIR: two blocks on neighbouring SMs to a tile, whose MMAs the first one issues for both.
+enum Mode { SINGLE, PAIR };
 
 template <Mode MODE>
 struct Sizes {
@@ -371,56 +371,40 @@ __device__ __forceinline__ Terms terms_of(const float (&v)[8]) {
     return t;
 }
 
-// What a cluster's blocks wrote is seen by all of them, their TMA fetches included.
-__device__ __forceinline__ void cluster_turn(bool wrote, bool fetches) {
+// Between two products: what any block wrote before is seen by all behind it, their TMA fetches included.  All blocks are resident (the
+// launch is a cooperative one), so each comes here; a block that has given up goes on without waiting.
+// (The warps of a block come here from different places.)
+__device__ __forceinline__ void block_barrier() { asm volatile("barrier.sync 1, %0;" ::"n"(TILE_THREADS) : "memory"); }
+__device__ __forceinline__ void all_blocks(u32* arrived, u32 due, volatile int* gave_up, int* timeout, bool wrote, bool fetches) {
     if (wrote) asm volatile("fence.proxy.async;" ::: "memory");
-    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    block_barrier();
+    if (threadIdx.x == 0 && gridDim.x > 1) {
+        __threadfence();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+        u64 t0 = 0;
+        for (u32 spins = 0; !*gave_up; ++spins) {
+            u32 n;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(arrived) : "memory");
+            if ((int)(n - due) >= 0) break;
+            if ((spins & 31u) == 31u) {
+                const u64 t = now_ns();
+                if (t0 == 0) t0 = t;
+                if (t - t0 > WAIT_NS || spins > (1u << 26)) {
+                    *gave_up = 1;
+                    *(volatile int*)timeout = 1;
+                }
+            }
+        }
+        __threadfence();
+    }
+    block_barrier();
     if (fetches) asm volatile("fence.proxy.async;" ::: "memory");
 }
 
-// In a cluster of `blocks`, all threads: momentum, norm and X, split, of one matrix.
-__device__ __forceinline__ void start_in_cluster(const Jobs& p, const Shape& q, int b, int rank, int blocks, double* s_part) {
-    const int rows = q.turned ? q.n : q.m, cols = q.turned ? q.m : q.n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double s = 0.0;
-    for (int i = rank * (TILE_THREADS / 32) + warp; i < rows; i += blocks * (TILE_THREADS / 32))
-        for (int c = lane; c < cols; c += 32) {
-            if (q.of.m) {
-                float* m = &q.of.m[i * q.of.ldm + c];
-                *m = p.momentum * *m + q.of.g[i * q.of.ldg + c];
-            }
-            const double u = update_at(p, q, b, i, c);
-            s += u * u;
-        }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) s_part[warp] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < TILE_THREADS / 32; ++i) s += s_part[i];
-        __stcg(&q.parts[b * PARTS + rank], s);
-    }
-    cluster_turn(false, false);
-    s = 0.0;
-    for (int i = 0; i < blocks; ++i) s += __ldcg(&q.parts[b * PARTS + i]);
-    const double scale = (double)SCALE / (sqrt(s) + (double)p.eps);
-    const int64_t plane = (int64_t)q.m * q.ldx;
-    __half* x = q.px[0] + 2 * b * plane;
-    for (int i = rank * (TILE_THREADS / 32) + warp; i < rows; i += blocks * (TILE_THREADS / 32))
-        for (int c = lane; c < cols; c += 32) {
-            __half h, l;
-            split((float)((double)update_at(p, q, b, i, c) * scale), h, l);
-            const int64_t at = q.turned ? (int64_t)c * q.ldx + i : (int64_t)i * q.ldx + c;
-            x[at] = h;
-            x[at + plane] = l;
-        }
-    cluster_turn(true, true);
-}
-
-// One kind of product over the tiles of all matrices; or, with CLUSTER, all products of one.
+// All products of all matrices, one kind after the other: as launches of their own each of the fifteen took 5 to 8 us before its first MMA.
 template <Mode MODE>
-__global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const Kind only, const int first_from,
-                                                                  const int all_tiles, const bool only_last, const int steps) {
+__global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const int sym_tiles, const int all_tiles,
+                                                                  const int steps) {
     using S = Sizes<MODE>;
     constexpr int BN = S::BN;
     constexpr bool TWO = MODE == PAIR;
@@ -428,7 +412,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
     __shared__ u64 s_bar[2 * S::STAGES + 2 * S::ACCS + 1];
     __shared__ u32 s_tmem;
     __shared__ int s_gave_up;
-    __shared__ double s_norm[MODE == CLUSTER ? TILE_THREADS / 32 : 1];
     // (at an index that is not known beforehand, parameters are read from the constant bank at hundreds of cycles a time)
     __shared__ Shape s_jobs[MAX_JOBS];
     const u32 smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -461,34 +444,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         rank >>= 1, stride >>= 1;
     }
     auto wait = [&](u32 bar, u32 parity) { return warp_wait(bar, parity, gave_up, p.timeout); };
-    Where one{0, 0, 0, 0};
-    if constexpr (MODE == CLUSTER) {
-        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-        asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(stride));
-        one.matrix = blockIdx.x / stride;
-        while (one.matrix >= s_jobs[one.job].batch) one.matrix -= s_jobs[one.job++].batch;
-        start_in_cluster(p, s_jobs[one.job], one.matrix, rank, stride, s_norm);
-    }
-    // f(kind, the buffer X is in, whether it is the last product): in a cluster all blocks go from one product to the next together,
-    // those that have given up, too.
+    // f(kind, the buffer X is in, whether it is the last product)
     auto each_product = [&](auto&& f) {
-        if constexpr (MODE != CLUSTER) {
-            f(only, first_from, only_last);
-        } else {
-            for (int k = 0; k < steps; ++k)
-                for (int kind = GRAM; kind <= APPLY; ++kind) {
-                    f((Kind)kind, k & 1, k + 1 == steps);
-                    if (kind != APPLY || k + 1 < steps) cluster_turn(warp < PRODUCER, warp == PRODUCER);
-                }
-        }
+        u32 due = 0;
+        for (int k = 0; k < steps; ++k)
+            for (int kind = GRAM; kind <= APPLY; ++kind) {
+                f((Kind)kind, k & 1, k + 1 == steps);
+                due += gridDim.x;
+                if (kind != APPLY || k + 1 < steps) all_blocks(p.arrived, due, gave_up, p.timeout, warp < PRODUCER, warp == PRODUCER);
+            }
     };
-    auto tiles_of = [&](Kind kind) { return MODE != CLUSTER ? all_tiles : kind == APPLY ? s_jobs[one.job].tiles_all : s_jobs[one.job].tiles_sym; };
-    auto find = [&](Kind kind, int t) {
-        if constexpr (MODE != CLUSTER) return tile_of<S::ROWS, BN>(s_jobs, kind, t);
-        Where w = one;
-        place<S::ROWS, BN>(s_jobs[w.job], kind, t, w);
-        return w;
-    };
+    auto tiles_of = [&](Kind kind) { return kind == APPLY ? all_tiles : sym_tiles; };
 
     if (warp == PRODUCER) {
         const u32 first_full = TWO ? in_first(full) : full;
@@ -496,7 +462,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         bool ok = true;
         each_product([&](Kind kind, int from, bool) {
           for (int t = rank; t < tiles_of(kind) && ok; t += stride) {
-            const Where w = find(kind, t);
+            const Where w = tile_of<S::ROWS, BN>(s_jobs, kind, t);
             const Shape& q = s_jobs[w.job];
             const int depth = kind == GRAM ? q.n : q.m;
             const Maps& maps = p.map[w.job];
@@ -529,7 +495,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         each_product([&](Kind kind, int, bool) {
           const u32 both = idesc_half(S::ROWS, 2 * BN, kind == APPLY), one_term = idesc_half(S::ROWS, BN, kind == APPLY);
           for (int t = rank; t < tiles_of(kind) && ok && side == 0; t += stride) {
-            const Where w = find(kind, t);
+            const Where w = tile_of<S::ROWS, BN>(s_jobs, kind, t);
             const Shape& q = s_jobs[w.job];
             const int depth = kind == GRAM ? q.n : q.m;
             for (int k = 0; k < depth; k += 64, ++it) {
@@ -566,7 +532,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         bool ok = true;
         each_product([&](Kind kind, int from, bool last) {
           for (int t = rank; t < tiles_of(kind) && ok; t += stride) {
-            const Where w = find(kind, t);
+            const Where w = tile_of<S::ROWS, BN>(s_jobs, kind, t);
             const Shape& q = s_jobs[w.job];
             const int depth = kind == GRAM ? q.n : q.m, width = kind == APPLY ? q.n : q.m, ld = kind == APPLY ? q.ldx : q.lda;
             float sum[EACH];
@@ -605,77 +571,91 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
             __half* to = (kind == GRAM ? q.pa : kind == SQUARE ? q.pb : q.px[from ^ 1]) + matrix;
             const __half* more = (kind == SQUARE ? q.pa : q.px[from]) + matrix;
             const float factor = kind == SQUARE ? QUINTIC_C * UNSCALE : UNSCALE, more_factor = kind == SQUARE ? QUINTIC_B : QUINTIC_A;
-            const bool result = kind == APPLY && last, turned = result && q.turned;
+            const bool result = kind == APPLY && last;
             const Matrix of = q.of;
             // 32 x 32 values at a time: as they were summed up a lane has a row; then it has eight neighbours of a row, four times.
-            const int row0 = S::ROWS * w.row + 128 * side + 32 * quarter, row = row0 + (lane >> 2);
+            const int row0 = S::ROWS * w.row + 128 * side + 32 * quarter, row = row0 + (lane >> 2), eighth = 8 * (lane & 3);
             Terms add[EACH / 32][4];
-            if (kind != GRAM) {
+            if (kind != GRAM) {  // (without a question about single ones, which would come one after the other; what lies outside is not used)
 #pragma unroll
-                for (int block = 0; block < EACH / 32; ++block)
+                for (int block = 0; block < EACH / 32; ++block) {
+                    const __half* at = more + min(BN * w.col + half * EACH + 32 * block + eighth, ld - 8);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int col = BN * w.col + half * EACH + 32 * block + 8 * (lane & 3);
-                        if (row + 8 * i < m && col < width) add[block][i].load(more + (int64_t)(row + 8 * i) * ld + col, plane);
-                    }
+                    for (int i = 0; i < 4; ++i) add[block][i].load(at + (int64_t)min(row + 8 * i, m - 1) * ld, plane);
+                }
             }
+            // Four columns of a row lie together in shared memory, those of row r at (column / 4) ^ (r & 7) ^ 2 (r / 8): no two lanes meet in
+            // a bank, by rows or by columns.
+            const int by_row = (lane >> 2) * 8, swirl = lane >> 2;
 #pragma unroll
             for (int block = 0; block < EACH / 32; ++block) {
-                const int col0 = BN * w.col + half * EACH + 32 * block, col = col0 + 8 * (lane & 3);
+                const int col0 = BN * w.col + half * EACH + 32 * block, col = col0 + eighth;
                 if (row0 >= m || col0 >= width || (kind != APPLY && col0 < row0)) continue;  // (below the diagonal: written across)
-                // Four columns of a row lie together, those of row r at (column / 4) ^ swirl(r): no two lanes meet in a bank, by rows or by
-                // columns.
-                auto swirl = [](int r) { return (r & 7) ^ (r >> 3 << 1); };
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    turn[lane * 8 + (c ^ swirl(lane))] = make_float4(sum[32 * block + 4 * c], sum[32 * block + 4 * c + 1], sum[32 * block + 4 * c + 2], sum[32 * block + 4 * c + 3]);
+                    turn[lane * 8 + (c ^ (lane & 7) ^ (lane >> 3 << 1))] =
+                        make_float4(sum[32 * block + 4 * c], sum[32 * block + 4 * c + 1], sum[32 * block + 4 * c + 2], sum[32 * block + 4 * c + 3]);
                 __syncwarp();
-                const bool across = kind != APPLY && col0 > row0;
+                auto values = [&](int i, float(&v)[8]) {
+                    const float4 x = turn[64 * i + by_row + ((eighth >> 2) ^ swirl ^ (2 * i))], y = turn[64 * i + by_row + (((eighth >> 2) + 1) ^ swirl ^ (2 * i))];
+                    v[0] = factor * x.x, v[1] = factor * x.y, v[2] = factor * x.z, v[3] = factor * x.w;
+                    v[4] = factor * y.x, v[5] = factor * y.y, v[6] = factor * y.z, v[7] = factor * y.w;
+                    if (kind != GRAM) add[block][i].add_to(v, more_factor);
+                };
+                auto put = [&](int i, uint4 x, uint4 y) {
+                    reinterpret_cast<uint4&>(turn[64 * i + by_row + ((eighth >> 2) ^ swirl ^ (2 * i))]) = x;
+                    reinterpret_cast<uint4&>(turn[64 * i + by_row + (((eighth >> 2) + 1) ^ swirl ^ (2 * i))]) = y;
+                };
+                // the same, turned: eight neighbours of a column, of the rows from 8 (lane % 4) on
+                auto turned_words = [&](int i, u32(&words)[8]) {
+                    const int column = 8 * i + (lane >> 2);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int in_row = 8 * i + (lane >> 2);
-                    float4 &lo = turn[in_row * 8 + ((2 * (lane & 3)) ^ swirl(in_row))], &hi = turn[in_row * 8 + ((2 * (lane & 3) + 1) ^ swirl(in_row))];
-                    const float4 x = lo, y = hi;
-                    float v[8] = {factor * x.x, factor * x.y, factor * x.z, factor * x.w, factor * y.x, factor * y.y, factor * y.z, factor * y.w};
-                    const bool in = row + 8 * i < m && col < width;
-                    if (kind != GRAM && in) add[block][i].add_to(v, more_factor);
-                    if (turned) {
-                        lo = make_float4(v[0], v[1], v[2], v[3]);
-                        hi = make_float4(v[4], v[5], v[6], v[7]);
-                    } else if (result) {
-                        if (in) of.write(w.matrix, row + 8 * i, col, min(8, width - col), v);
-                    } else {
+                    for (int j = 0; j < 8; ++j)
+                        words[j] = reinterpret_cast<const u32*>(turn)[(eighth + j) * 32 + (((column >> 2) ^ j ^ (2 * (lane & 3))) << 2) + (column & 3)];
+                };
+                const int r = row0 + eighth, c = col0 + (lane >> 2);
+                if (!result) {
+                    const bool across = kind != APPLY && col0 > row0;
+                    __half* out = to + (int64_t)row * ld + col;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i, out += 8 * ld) {
+                        float v[8];
+                        values(i, v);
                         const Terms t = terms_of(v);
-                        if (in) t.store(to + (int64_t)(row + 8 * i) * ld + col, plane);  // (the row's padding may be written over)
-                        if (across) {
-                            reinterpret_cast<uint4&>(lo) = make_uint4(t.word(0), t.word(1), t.word(2), t.word(3));
-                            reinterpret_cast<uint4&>(hi) = make_uint4(t.word(4), t.word(5), t.word(6), t.word(7));
-                        }
+                        if (row + 8 * i < m && col < width) t.store(out, plane);  // (the row's padding may be written over)
+                        if (across) put(i, make_uint4(t.word(0), t.word(1), t.word(2), t.word(3)), make_uint4(t.word(4), t.word(5), t.word(6), t.word(7)));
                     }
-                }
-                __syncwarp();
-                if (across || turned) {  // the same values, turned: eight neighbours of a column
-                    const int r = row0 + 8 * (lane & 3), c = col0 + (lane >> 2);
+                    if (across) {
+                        __syncwarp();
+                        out = to + (int64_t)c * ld + r;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int column = 8 * i + (lane >> 2);
-                        u32 words[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int at = 8 * (lane & 3) + j;
-                            words[j] = reinterpret_cast<const u32*>(turn)[at * 32 + (((column >> 2) ^ swirl(at)) << 2) + (column & 3)];
-                        }
-                        if (r >= m || c + 8 * i >= width) continue;
-                        if (across) {
+                        for (int i = 0; i < 4; ++i, out += 8 * ld) {
+                            u32 words[8];
+                            turned_words(i, words);
                             Terms t;
 #pragma unroll
                             for (int j = 0; j < 4; ++j) t.pair(j, words[2 * j], words[2 * j + 1]);
-                            t.store(to + (int64_t)(c + 8 * i) * ld + r, plane);
-                        } else {
+                            if (r < m && c + 8 * i < width) t.store(out, plane);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v[8];
+                        values(i, v);
+                        if (q.turned) put(i, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])), make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
+                        else if (row + 8 * i < m && col < width) of.write(w.matrix, row + 8 * i, col, min(8, width - col), v);
+                    }
+                    if (q.turned) {
+                        __syncwarp();
+#pragma unroll 1
+                        for (int i = 0; i < 4; ++i) {
+                            u32 words[8];
                             float v[8];
+                            turned_words(i, words);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(words[j]);
-                            of.write(w.matrix, c + 8 * i, r, min(8, m - r), v);
+                            if (r < m && c + 8 * i < width) of.write(w.matrix, c + 8 * i, r, min(8, m - r), v);
                         }
                     }
                 }
@@ -751,27 +731,9 @@ int tiles_all(int m, int n) {
 }
 
 template <Mode MODE>
-void launch(dim3 grid, int cluster, const cbm::Stream& on, const Jobs& p, Kind kind, int from, int tiles, bool last, int steps) {
-    cudaLaunchAttribute attrs[2] = {};
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim.x = cluster;
-    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = grid;
-    config.blockDim = dim3(TILE_THREADS);
-    config.dynamicSmemBytes = Sizes<MODE>::SMEM;
-    config.stream = on.s;
-    config.attrs = attrs;
-    config.numAttrs = on.captured ? 1 : 2;
-    (void)cudaLaunchKernelEx(&config, product_kernel<MODE>, p, kind, from, tiles, last, steps);
-}
-
-// A launch for every product, of all matrices.
-template <Mode MODE>
 int products(const char* who, Jobs& p, int steps, const cbm::Stream& on) {
-    if (!allow_smem<product_kernel<MODE>>(Sizes<MODE>::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
+    constexpr auto kernel = product_kernel<MODE>;
+    if (!allow_smem<kernel>(Sizes<MODE>::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
     int sym = 0, all = 0, matrices = 0, blocks = 1;
     for (int i = 0; i < p.count; ++i) {
         Shape& q = p.job[i];
@@ -782,30 +744,23 @@ int products(const char* who, Jobs& p, int steps, const cbm::Stream& on) {
     }
     cbm::launch_next(norm_kernel, dim3(PARTS, matrices), THREADS, 0, on, p);
     cbm::launch_next(start_kernel, dim3(blocks, matrices), THREADS, 0, on, p);
-    const int cluster = MODE == PAIR ? 2 : 1, most = sm_count() / cluster;
-    const dim3 for_sym((sym < most ? sym : most) * cluster), for_all((all < most ? all : most) * cluster);
-    for (int k = 0; k < steps; ++k) {
-        launch<MODE>(for_sym, cluster, on, p, GRAM, k & 1, sym, false, 0);
-        launch<MODE>(for_sym, cluster, on, p, SQUARE, k & 1, sym, false, 0);
-        launch<MODE>(for_all, cluster, on, p, APPLY, k & 1, all, k + 1 == steps, 0);
-    }
-    return CBM_B200_OK;
-}
-
-// One launch for everything, a cluster of blocks to a matrix.
-constexpr int CLUSTER_BLOCKS = 8, CLUSTER_TILES = 16;
-bool fits_cluster(int m, int n) { return tiles_sym<CLUSTER>(m) <= CLUSTER_BLOCKS && tiles_all<CLUSTER>(m, n) <= CLUSTER_TILES; }
-
-int clusters(const char* who, Jobs& p, int steps, const cbm::Stream& on) {
-    if (!allow_smem<product_kernel<CLUSTER>>(Sizes<CLUSTER>::SMEM)) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no room in shared memory");
-    int matrices = 0;
-    for (int i = 0; i < p.count; ++i) {
-        Shape& q = p.job[i];
-        q.tiles_sym = tiles_sym<CLUSTER>(q.m), q.tiles_all = tiles_all<CLUSTER>(q.m, q.n);
-        matrices += q.batch;
-    }
-    launch<CLUSTER>(dim3(matrices * CLUSTER_BLOCKS), CLUSTER_BLOCKS, on, p, GRAM, 0, 0, false, steps);
-    return CBM_B200_OK;
+    const int cluster = MODE == PAIR ? 2 : 1, most = sm_count() / cluster, wanted = sym > all ? sym : all;
+    cudaLaunchAttribute attrs[2] = {};
+    attrs[0].id = cudaLaunchAttributeCooperative;
+    attrs[0].val.cooperative = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = cluster;
+    attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((wanted < most ? wanted : most) * cluster);
+    config.blockDim = dim3(TILE_THREADS);
+    config.dynamicSmemBytes = Sizes<MODE>::SMEM;
+    config.stream = on.s;
+    config.attrs = attrs;
+    config.numAttrs = MODE == PAIR ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p, sym, all, steps);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
 int run(const char* who, Jobs& p, int steps, void* stream) {
@@ -813,7 +768,6 @@ int run(const char* who, Jobs& p, int steps, void* stream) {
     p.timeout = timeout_word();
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
     int64_t pairs = 0;
-    bool small = true;
     for (int i = 0; i < p.count; ++i) {
         Shape& q = p.job[i];
         Maps& map = p.map[i];
@@ -824,21 +778,21 @@ int run(const char* who, Jobs& p, int steps, void* stream) {
         if (!done)
             return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no tensor map for its operands");
         pairs += (int64_t)q.batch * tiles_sym<PAIR>(q.m);
-        small = small && fits_cluster(q.m, q.n);
     }
     // Pairs of blocks where there are tiles of 256 x 128 for half of them at least, else single ones.
-    const int rc = small ? clusters(who, p, steps, on) : pairs * 4 >= sm_count() ? products<PAIR>(who, p, steps, on) : products<SINGLE>(who, p, steps, on);
+    const int rc = pairs * 4 >= sm_count() ? products<PAIR>(who, p, steps, on) : products<SINGLE>(who, p, steps, on);
     if (rc) return rc;
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
+constexpr int HEAD = 256;  // of a workspace: the count of blocks
 constexpr int MAX_SIDE = 1 << 16, MAX_BATCH = 32768;  // (tiles are counted in 31 bits, matrices in a grid's second dimension)
 
 }  // namespace
 
 extern "C" int64_t cbm_b200_orthogonalise_workspace(int32_t batch, int32_t rows, int32_t cols) {
-    return batch > 0 && rows > 0 && cols > 0 ? lay_out(nullptr, rows, cols, batch, nullptr) : 0;
+    return batch > 0 && rows > 0 && cols > 0 ? HEAD + lay_out(nullptr, rows, cols, batch, nullptr) : 0;
 }
 
 extern "C" int cbm_b200_orthogonalise(const float* u, int64_t ldu, int64_t next_u, float* out, int64_t ldout, int64_t next_out, int32_t batch,
@@ -852,7 +806,8 @@ extern "C" int cbm_b200_orthogonalise(const float* u, int64_t ldu, int64_t next_
     if (workspace_bytes < cbm_b200_orthogonalise_workspace(batch, rows, cols)) return cbm::fail(CBM_B200_ERR_ARG, "orthogonalise: workspace too small");
     Jobs p{};
     p.count = 1, p.eps = eps;
-    lay_out(&p.job[0], rows, cols, batch, static_cast<unsigned char*>(workspace));
+    p.arrived = static_cast<u32*>(workspace);
+    lay_out(&p.job[0], rows, cols, batch, static_cast<unsigned char*>(workspace) + HEAD);
     p.job[0].of = Matrix{u, nullptr, nullptr, out, ldu, 0, 0, ldout, next_u, next_out, 0.f, 0.f};
     return run("orthogonalise", p, steps, stream);
 }
@@ -861,7 +816,7 @@ extern "C" int64_t cbm_b200_orthogonal_step_workspace(const cbm_b200_update_of* 
     int64_t all = 0;
     for (int i = 0; of && i < count; ++i)
         if (of[i].rows > 0 && of[i].cols > 0) all += lay_out(nullptr, of[i].rows, of[i].cols, 1, nullptr);
-    return all;
+    return all ? HEAD + all : 0;
 }
 
 extern "C" int cbm_b200_orthogonal_step(const cbm_b200_update_of* of, int32_t count, float lr, float momentum, int32_t nesterov,
@@ -877,23 +832,20 @@ extern "C" int cbm_b200_orthogonal_step(const cbm_b200_update_of* of, int32_t co
     const int64_t need = cbm_b200_orthogonal_step_workspace(of, count);
     if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need))
         return cbm::fail(CBM_B200_ERR_ARG, "orthogonal_step: workspace too small, or not at 256 bytes");
-    unsigned char* at = static_cast<unsigned char*>(workspace);
-    // Those that a cluster of blocks does by itself, and the others.
-    for (int small = 1; small >= 0; --small)
-        for (int i = 0; i < count;) {
-            Jobs p{};
-            p.eps = eps, p.momentum = momentum, p.nesterov = nesterov;
-            for (; i < count && p.count < MAX_JOBS; ++i) {
-                const cbm_b200_update_of& u = of[i];
-                const int m = u.rows < u.cols ? u.rows : u.cols, n = u.rows < u.cols ? u.cols : u.rows;
-                if (m == 0 || fits_cluster(m, n) != (small != 0)) continue;
-                Shape& q = p.job[p.count++];
-                at += lay_out(&q, u.rows, u.cols, 1, at);
-                const double tall = u.rows > u.cols ? std::sqrt((double)u.rows / u.cols) : 1.0;
-                q.of = Matrix{u.g, u.m, u.w, nullptr, u.ldg, u.ldm, u.ldw, 0, 0, 0, (float)(lr * tall), (float)(1.0 - (double)lr * weight_decay)};
-            }
-            if (p.count)
-                if (int rc = run("orthogonal_step", p, steps, stream)) return rc;
+    unsigned char* at = static_cast<unsigned char*>(workspace) + HEAD;
+    for (int i = 0; i < count;) {
+        Jobs p{};
+        p.eps = eps, p.momentum = momentum, p.nesterov = nesterov, p.arrived = static_cast<u32*>(workspace);
+        for (; i < count && p.count < MAX_JOBS; ++i) {
+            const cbm_b200_update_of& u = of[i];
+            if (u.rows == 0 || u.cols == 0) continue;
+            Shape& q = p.job[p.count++];
+            at += lay_out(&q, u.rows, u.cols, 1, at);
+            const double tall = u.rows > u.cols ? std::sqrt((double)u.rows / u.cols) : 1.0;
+            q.of = Matrix{u.g, u.m, u.w, nullptr, u.ldg, u.ldm, u.ldw, 0, 0, 0, (float)(lr * tall), (float)(1.0 - (double)lr * weight_decay)};
         }
+        if (p.count)
+            if (int rc = run("orthogonal_step", p, steps, stream)) return rc;
+    }
     return CBM_B200_OK;
 }
