@@ -9,10 +9,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .dense import _call, _ld, _rows
-from .norm import TYPES, rows_like
+from .norm import TYPES, _data, needs_function, only_once, rows_like
 
 MAX_TOP = 32  # include/cbm_b200.h, CBM_B200_MAX_TOP
 
@@ -24,33 +23,39 @@ class ClassLogProbs(NamedTuple):
     top_classes: torch.Tensor     # [N, top] int64; of equal logits the lower class comes first
 
 
+def _forward(x, labels, top, keep):
+    n, c = x.shape
+    log_prob = torch.empty(n, dtype=torch.float32, device=x.device)
+    entropy = torch.empty_like(log_prob)
+    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+    best = torch.empty((n, top), dtype=torch.float32, device=x.device)
+    classes = torch.empty((n, top), dtype=torch.int64, device=x.device)
+    _call("cbm_b200_class_log_probs", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(), labels.dtype is torch.int64, n, c, top,
+          log_prob.data_ptr(), entropy.data_ptr(), _data(stats), best.data_ptr(), classes.data_ptr())
+    return log_prob, entropy, best, classes, stats
+
+
 class _ClassLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, top):
-        x, n, c = _rows(logits), logits.size(0), logits.size(1)
-        labels = labels.contiguous()
-        new = dict(dtype=torch.float32, device=x.device)
-        log_prob, entropy, stats = torch.empty(n, **new), torch.empty(n, **new), torch.empty((n, 2), **new)
-        best, classes = torch.empty((n, top), **new), torch.empty((n, top), dtype=torch.int64, device=x.device)
-        _call("cbm_b200_class_log_probs", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(),
-              int(labels.dtype == torch.int64), n, c, top, log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), best.data_ptr(),
-              classes.data_ptr())
+    def forward(ctx, x, labels, top):
+        log_prob, entropy, best, classes, stats = _forward(x, labels, top, True)
         ctx.save_for_backward(x, labels, stats, entropy, classes)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(classes)
         return log_prob, entropy, best, classes
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_log, g_entropy, g_top, _):
-        x, labels, stats, entropy, classes = ctx.saved_tensors
-        x, labels, stats, entropy, classes = _rows(x), labels.contiguous(), stats.contiguous(), entropy.contiguous(), classes.contiguous()
-        given = [None if g is None else g.contiguous() for g in (g_log, g_entropy, g_top)]
-        n, c = x.size(0), x.size(1)
+    @only_once
+    def backward(ctx, *grads):
+        x, *kept = ctx.saved_tensors
+        # (a saved-tensor hook may hand them back in another layout)
+        x = _rows(x)
+        labels, stats, entropy, classes = (t.contiguous() for t in kept)
+        g_log, g_entropy, g_top = (None if g is None else g.contiguous() for g in grads[:3])
+        n, c = x.shape
         gx = rows_like(x)
-        _call("cbm_b200_class_log_probs_grad", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(),
-              int(labels.dtype == torch.int64), n, c, classes.size(1), stats.data_ptr(), entropy.data_ptr(), classes.data_ptr(),
-              *(None if g is None else g.data_ptr() for g in given), gx.data_ptr(), _ld(gx))
+        _call("cbm_b200_class_log_probs_grad", x.get_device(), x.data_ptr(), _ld(x), TYPES[x.dtype], labels.data_ptr(), labels.dtype is torch.int64, n, c,
+              classes.size(1), stats.data_ptr(), entropy.data_ptr(), classes.data_ptr(), _data(g_log), _data(g_entropy), _data(g_top), gx.data_ptr(),
+              _ld(gx))
         return gx, None, None
 
 
@@ -80,16 +85,20 @@ def class_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0) ->
     class; a row without an open class has log probabilities -inf, entropy 0 and no gradient.  A row with NaN or +inf is
     NaN throughout.  Differentiable once in ``logits``, through all three results.
     """
-    if logits.dim() != 2 or logits.size(1) < 1 or labels.shape != logits.shape[:1]:
-        raise RuntimeError(f"class log probabilities: shape mismatch, logits of {tuple(logits.shape)} and labels of {tuple(labels.shape)}")
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] < 1 or labels.shape != shape[:1]:
+        raise RuntimeError(f"class log probabilities: shape mismatch, logits of {tuple(shape)} and labels of {tuple(labels.shape)}")
     if logits.dtype not in TYPES:
         raise RuntimeError(f"class log probabilities: fp32, bf16 or fp16 logits expected, not {logits.dtype}")
-    if labels.dtype not in (torch.int64, torch.int32):
+    if labels.dtype is not torch.int64 and labels.dtype is not torch.int32:
         raise RuntimeError(f"class log probabilities: int64 or int32 labels expected, not {labels.dtype}")
     if labels.device != logits.device:
         raise RuntimeError(f"class log probabilities: logits on {logits.device} and labels on {labels.device}")
-    if not 0 <= top <= min(MAX_TOP, logits.size(1)):
-        raise ValueError(f"top must be between 0 and {min(MAX_TOP, logits.size(1))}")
+    if not 0 <= top <= min(MAX_TOP, shape[1]):
+        raise ValueError(f"top must be between 0 and {min(MAX_TOP, shape[1])}")
     if not logits.is_cuda:
         return _on_host(logits, labels, top)
-    return ClassLogProbs(*_ClassLogProbs.apply(logits, labels, int(top)))
+    x, labels = _rows(logits), labels.contiguous()
+    if needs_function(x):
+        return ClassLogProbs(*_ClassLogProbs.apply(x, labels, int(top)))
+    return ClassLogProbs(*_forward(x, labels, int(top), False)[:4])

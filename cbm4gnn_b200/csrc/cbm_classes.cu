@@ -61,8 +61,7 @@ __device__ __forceinline__ void store_row(const ForwardParams& p, int64_t row, c
     const int64_t label = label_of(p.labels, p.wide_labels, row);
     p.log_prob[row] = label < 0 ? 0.f : label >= p.c ? NAN : m == -INFINITY ? -INFINITY : (cbm::widen(x[label]) - m) - ls;
     p.entropy[row] = entropy;
-    p.stats[2 * row] = m;
-    p.stats[2 * row + 1] = ls;
+    if (p.stats) *reinterpret_cast<float2*>(p.stats + 2 * row) = float2{m, ls};
 }
 
 // Rows of up to 32 VALUES classes that are wide, or lie at odd places: `lanes` neighbouring lanes to a row (a power of two), which hold
@@ -806,7 +805,7 @@ extern "C" int cbm_b200_class_log_probs(const void* logits, int64_t ld, int32_t 
                                         float* top_log_prob, int64_t* top_class, void* stream) {
     if (int rc = check("class_log_probs", n_rows, ld, n_classes, top, type)) return rc;
     if (n_rows == 0) return CBM_B200_OK;
-    if (!logits || !labels || !log_prob || !entropy || !stats || (top && (!top_log_prob || !top_class)))
+    if (!logits || !labels || !log_prob || !entropy || (top && (!top_log_prob || !top_class)))
         return cbm::fail(CBM_B200_ERR_ARG, "class_log_probs: NULL argument");
     ForwardParams p{logits, labels, ld, n_rows, n_classes, top, wide_labels, 1, 0, log_prob, entropy, stats, top_log_prob, top_class};
     const cbm::Stream on(static_cast<cudaStream_t>(stream));

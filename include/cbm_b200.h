@@ -368,7 +368,7 @@ int cbm_b200_spmm_update_static(cbm_b200_plan* p, const float* x, int64_t ldx, f
  *                                probability of its label, the entropy of the row, and its `top` most probable
  *                                classes with their log probabilities (equal logits: lower class first; top <= n_classes).
  *                                labels [dev]: int64 where wide_labels, else int32; negative: none (log probability 0);
- *                                n_classes or more: NaN.  stats [dev, 2 x n_rows] is for the gradient.
+ *                                n_classes or more: NaN.  stats [dev, 2 x n_rows, 8-byte aligned] is for the gradient, or NULL.
  *                                top_log_prob, top_class [dev, n_rows x top].
  * cbm_b200_class_log_probs_grad  dx [dev, type of the logits] from the gradients of log_prob [n_rows], entropy [n_rows] and
  *                                top_log_prob [n_rows x top], of which any may be NULL; stats, entropy and top_class as the
