@@ -42,6 +42,7 @@ struct Params {
     int64_t tile, tiles;        // rows to a tile; tiles
     int team, slab_groups, lanes;    // threads of a team; groups of a column slab; threads of a group
     float2 *pieces, *joined;    // [2][groups][tiles], [tiles][groups]
+    int64_t* longer;            // [2][tiles]: the samples that pieces are of, -1: none
     float2* channels;           // [tiles][c]: sums of g xh and g
     int64_t parts;              // of `channels`
 };
@@ -52,15 +53,24 @@ __device__ __forceinline__ float param(const void* w, int wide, int c, float non
 }
 
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-__device__ __forceinline__ float activated(float z, int act) {
-    if (act == CBM_B200_ACT_RELU) return z <= 0.f ? 0.f : z;  // NaN passes
-    return act == CBM_B200_ACT_SILU ? z * sigmoid(z) : z;
+template <int ACT>
+__device__ __forceinline__ float activated(float z) {
+    if constexpr (ACT == CBM_B200_ACT_RELU) return z <= 0.f ? 0.f : z;  // NaN passes
+    return ACT == CBM_B200_ACT_SILU ? z * sigmoid(z) : z;
 }
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == CBM_B200_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
-    if (act != CBM_B200_ACT_SILU) return 1.f;
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == CBM_B200_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
+    if constexpr (ACT != CBM_B200_ACT_SILU) return 1.f;
     const float s = sigmoid(z);
     return s * (1.f + z * (1.f - s));
+}
+// Calls f with the activation as a constant: asked for value by value it costs as much as the rest.
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+    if (act == CBM_B200_ACT_SILU) f(std::integral_constant<int, CBM_B200_ACT_SILU>());
+    else if (act == CBM_B200_ACT_RELU) f(std::integral_constant<int, CBM_B200_ACT_RELU>());
+    else f(std::integral_constant<int, CBM_B200_ACT_NONE>());
 }
 
 // The E values of a group that fall to a thread in each row.  Where rows and groups allow it they are one vector of up to 16 bytes; else
@@ -74,9 +84,9 @@ struct Values {
     __device__ Values() {}
     __device__ __forceinline__ void load(const T* p, int lanes, int there) {
         if constexpr (STRIDED) {
+            // (the first again in place of a missing one, which is not used: a branch for each would make them wait for one another)
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (i < there) v[i] = p[i * lanes];
+            for (int i = 0; i < E; ++i) v[i] = p[i < there ? i * lanes : 0];
         } else {
             bits = *reinterpret_cast<const decltype(bits)*>(p);
         }
@@ -180,20 +190,24 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowSha
         const float r = rsqrtf(group_sum(s, h, s_warp).x * share + p.eps);
         V out;
         if constexpr (!GRAD) {
+            with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(activated(x[i] * (r * w[i]) + b[i], p.act));
+                for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(activated<decltype(act)::value>(x[i] * (r * w[i]) + b[i]));
+            });
         } else {
             s.x = 0.f;
+            with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                x[i] *= r;
-                const float g = u[i] * slope(x[i] * w[i] + b[i], p.act);
-                gw[i] += g * x[i];
-                gb[i] += g;
-                u[i] = g * w[i];
-                s.x += u[i];
-                s.y += u[i] * x[i];
-            }
+                for (int i = 0; i < E; ++i) {
+                    x[i] *= r;
+                    const float g = u[i] * slope<decltype(act)::value>(x[i] * w[i] + b[i]);
+                    gw[i] += g * x[i];
+                    gb[i] += g;
+                    u[i] = g * w[i];
+                    s.x += u[i];
+                    s.y += u[i] * x[i];
+                }
+            });
             s = group_sum(s, h, s_warp);
 #pragma unroll
             for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(r * (u[i] - s.x * share - x[i] * (s.y * share)));
@@ -226,26 +240,30 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowSha
 __device__ __forceinline__ int64_t start_of(const Params& p, int64_t s) {
     return p.ptr ? min(max(p.ptr[s], (int64_t)0), p.n_rows) : s * p.rows_each;
 }
-// The last sample that starts at `row` or before it, -1: none.  The lanes of a warp try 32 places at a time.
-__device__ __forceinline__ int64_t sample_at(const Params& p, int64_t row) {
-    if (!p.ptr) return p.rows_each ? min(row / p.rows_each, p.n_samples - 1) : p.n_samples - 1;
-    const int lane = threadIdx.x & 31;
+// The last samples that start at `row` and at `other` or before them, -1: none.  Half a warp's lanes each try 16 places at a time.
+__device__ __forceinline__ void samples_at(const Params& p, int64_t row, int64_t other, int64_t& s, int64_t& t) {
+    if (!p.ptr) {
+        s = p.rows_each ? min(row / p.rows_each, p.n_samples - 1) : p.n_samples - 1;
+        t = p.rows_each ? min(other / p.rows_each, p.n_samples - 1) : p.n_samples - 1;
+        return;
+    }
+    const int lane = threadIdx.x & 15, upper = threadIdx.x & 16;
+    if (upper) row = other;
     int64_t lo = 0, hi = p.n_samples + 1;  // entries before lo are <= row, those from hi on are larger
-    while (lo < hi) {
-        const int64_t each = (hi - lo + 31) / 32, probe = lo + each * lane + each - 1;
-        const bool below = probe < hi && p.ptr[probe] <= row;
-        const int n = __popc(__ballot_sync(FULL, below));
+    while (__any_sync(FULL, lo < hi)) {
+        const int64_t each = (hi - lo + 15) / 16, probe = lo + each * lane + each - 1;
+        const bool below = lo < hi && probe < hi && p.ptr[probe] <= row;
+        const int n = __popc(__ballot_sync(FULL, below) >> upper & 0xffffu);
         const int64_t from = lo;
         lo = min(from + each * n, hi);
-        hi = min(hi, from + each * (n + 1) - 1);
-        if (hi < lo) hi = lo;
+        hi = max(lo, min(hi, from + each * (n + 1) - 1));
     }
-    return lo - 1;
+    s = __shfl_sync(FULL, lo, 0) - 1;
+    t = __shfl_sync(FULL, lo, 16) - 1;
 }
-// Where the tile that should start at `row` does: samples that are no longer than a tile are not cut.
-__device__ __forceinline__ int64_t tile_start(const Params& p, int64_t row) {
+// Where the tile that should start at `row`, where sample s lies, does: samples that are no longer than a tile are not cut.
+__device__ __forceinline__ int64_t tile_start(const Params& p, int64_t row, int64_t s) {
     if (row >= p.n_rows) return p.n_rows;
-    const int64_t s = sample_at(p, row);
     if (s < 0 || s >= p.n_samples) return row;
     const int64_t a = start_of(p, s), e = start_of(p, s + 1);
     return row < e && e - a <= p.tile ? a : row;
@@ -277,85 +295,135 @@ struct Team {
     }
 };
 
-// Joins what the threads of a team found in `rows` rows into one result for each group.  f(group, sum of the two values) is called
-// by a lane for each group.  MEANS: the values are the mean over a thread's values of all its rows and the squares around it.
-template <bool MEANS, int E, bool STRIDED, class F>
-__device__ __forceinline__ void join_groups(const Params& p, const Team& t, const float2* part, int rows, F&& f) {
-    const int warp = t.thread >> 5, lane = t.thread & 31, entries = min(t.at_once, rows) * p.lanes;
-    for (int g = warp; g < t.groups; g += t.size >> 5) {
-        const float2* first = part + g * p.lanes;
-        if constexpr (MEANS) {
-            const float ref = first[0].x;
-            // f(what a thread left, how many values it is of)
-            auto each = [&](auto&& f) {
-                for (int i = lane; i < entries; i += 32) {
-                    const int r = i / p.lanes, l = i - r * p.lanes, n = (rows - r + t.at_once - 1) / t.at_once;
-                    f(first[r * t.vectors + l], (float)(n * values_of<E, STRIDED>(l, p.lanes, p.width)));
-                }
-            };
-            float s = 0.f;
-            each([&](float2 one, float n) { s += n * (one.x - ref); });
-            const float mean = ref + lanes_sum(s, 32) / ((float)rows * (float)p.width);
-            s = 0.f;
-            each([&](float2 one, float n) { s += one.y + n * (one.x - mean) * (one.x - mean); });
-            s = lanes_sum(s, 32);
-            if (lane == 0) f(g, float2{mean, s});
-        } else {
-            float2 s{0.f, 0.f};
-            for (int i = lane; i < entries; i += 32) {
-                const int r = i / p.lanes;
-                const float2 one = first[r * t.vectors + i - r * p.lanes];
-                s.x += one.x, s.y += one.y;
-            }
-            s.x = lanes_sum(s.x, 32), s.y = lanes_sum(s.y, 32);
-            if (lane == 0) f(g, s);
+// What two parts of a group come to: the mean of all values and the squares around it, or (not MEANS) sums of two values.  `part` holds
+// what each thread of a team found in `rows` rows: the mean over its values of all its rows and the squares around it, or its sums.
+template <bool MEANS, int E, bool STRIDED>
+struct Join {
+    const Params& p;
+    const Team& t;
+    const float2* part;  // of the group
+    int rows;
+    // Rows of thread r of those that are at work on a column.
+    __device__ __forceinline__ int rows_of(int r) const { return (rows - r + t.at_once - 1) / t.at_once; }
+    // By one thread: f(what a thread left, how many values it is of).
+    template <class F>
+    __device__ __forceinline__ void alone(F&& f) const {
+        const int most = min(t.at_once, rows);
+        const float2* at = part;
+        for (int r = 0; r < most; ++r, at += t.vectors) {
+            const int n = rows_of(r);
+            const float full = (float)(n * E);
+            for (int l = 0; l < p.lanes; ++l) f(at[l], STRIDED ? (float)(n * values_of<E, STRIDED>(l, p.lanes, p.width)) : full);
         }
+    }
+    // By a warp.
+    template <class F>
+    __device__ __forceinline__ void together(F&& f) const {
+        const int entries = min(t.at_once, rows) * p.lanes;
+        for (int i = threadIdx.x & 31; i < entries; i += 32) {
+            const int r = i / p.lanes, l = i - r * p.lanes;
+            f(part[r * t.vectors + l], (float)(rows_of(r) * values_of<E, STRIDED>(l, p.lanes, p.width)));
+        }
+    }
+    template <bool WARP>
+    __device__ __forceinline__ float2 run() const {
+        float2 s{0.f, 0.f};
+        auto each = [&](auto&& f) {
+            if constexpr (WARP) together(f);
+            else alone(f);
+        };
+        auto sum = [&](float v) { return WARP ? lanes_sum(v, 32) : v; };
+        if constexpr (MEANS) {
+            const float ref = part[0].x;
+            each([&](float2 one, float n) { s.x += n * (one.x - ref); });
+            s.x = ref + sum(s.x) / ((float)rows * (float)p.width);
+            each([&](float2 one, float n) { s.y += one.y + n * (one.x - s.x) * (one.x - s.x); });
+            s.y = sum(s.y);
+        } else {
+            each([&](float2 one, float) { s.x += one.x, s.y += one.y; });
+            s = float2{sum(s.x), sum(s.y)};
+        }
+        return s;
+    }
+};
+// A group of few threads is joined by each of them for itself, which saves the way through shared memory and a barrier.
+constexpr int FEW = 32;
+
+// A number of rows that is known beforehand.
+template <int N>
+struct All {
+    __device__ __forceinline__ constexpr operator int() const { return N; }
+};
+// Rows that a thread fetches at a time.
+template <class T, int E, bool STRIDED, bool GRAD>
+__host__ __device__ constexpr int batch_of() {
+    return STRIDED ? (E == 1 ? 8 : E == 4 || !GRAD ? 4 : 2) : E * sizeof(T) >= 8 ? 4 : 8;
+}
+// Calls f(values, values of the gradient, how many rows) for the `count` rows from x on, `dx` apart, a batch at a time.  The last rows are
+// fetched without a question about each, the last one again in place of those that are not there: as branches the fetches would come
+// one after the other.
+template <class T, int E, bool STRIDED, bool GRAD, class F>
+__device__ __forceinline__ void for_rows(const T* x, const T* gy, int64_t dx, int64_t dg, int64_t count, int lanes, int there, F&& f) {
+    constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
+    Values<T, E, STRIDED> v[BATCH], g[GRAD ? BATCH : 1];
+    for (; count >= BATCH; count -= BATCH) {
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            v[k].load(x, lanes, there), x += dx;
+            if constexpr (GRAD) g[k].load(gy, lanes, there), gy += dg;
+        }
+        f(v, g, All<BATCH>());
+    }
+    if (count > 0) {
+        const int have = (int)count;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            v[k].load(x, lanes, there);
+            if constexpr (GRAD) g[k].load(gy, lanes, there);
+            if (k + 1 < have) x += dx, gy += dg;
+        }
+        f(v, g, have);
     }
 }
 
-// Rows [lo, hi) of a sample: y, or gx, from the statistics (mean, r) and, for the gradient, the means of u and u xh; from the last row
-// to the first where BACK.
+// y, or gx, from the statistics (mean, r) and, for the gradient, the means of u and u xh.
+template <class T, int E, bool STRIDED, bool GRAD, int ACT>
+__device__ __forceinline__ Values<T, E, STRIDED> finished(const Values<T, E, STRIDED>& x, const Values<T, E, STRIDED>& gy, const float (&w)[E],
+                                                          const float (&b)[E], float2 stat, float2 sums) {
+    Values<T, E, STRIDED> to;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float d = cbm::widen(x.v[i]) - stat.x, z = d * (stat.y * w[i]) + b[i];
+        if constexpr (GRAD) {
+            const float u = cbm::widen(gy.v[i]) * slope<ACT>(z) * w[i];
+            to.v[i] = cbm::narrow<T>(stat.y * (u - sums.x - d * stat.y * sums.y));
+        } else {
+            to.v[i] = cbm::narrow<T>(activated<ACT>(z));
+        }
+    }
+    return to;
+}
+
+// Rows [lo, hi) of a sample, from the last row to the first where BACK.
 template <class T, int E, bool STRIDED, bool GRAD, bool BACK>
 __device__ __forceinline__ void write_rows(const Params& p, const Team& t, int64_t lo, int64_t hi, const float (&w)[E], const float (&b)[E],
                                            float2 stat, float2 sums) {
     const int64_t first = lo + t.row_in;
     if (!t.on() || first >= hi) return;
     const int64_t count = (hi - first + t.at_once - 1) / t.at_once;
-    constexpr int BATCH = E == 8 ? 2 : 4;
     const int64_t begin = BACK ? first + (count - 1) * t.at_once : first, step = BACK ? -t.at_once : t.at_once;
-    const T *x = static_cast<const T*>(p.x) + t.channel + begin * p.ldx, *gy = static_cast<const T*>(p.gy) + t.channel + begin * p.ldgy;
     T* y = static_cast<T*>(p.y) + t.channel + begin * p.ldy;
-    const int64_t dx = step * p.ldx, dg = step * p.ldgy, dy = step * p.ldy;
-    float rw[E];
+    const int64_t dy = step * p.ldy;
+    with_activation(p.act, [&](auto act) {
+        for_rows<T, E, STRIDED, GRAD>(static_cast<const T*>(p.x) + t.channel + begin * p.ldx, static_cast<const T*>(p.gy) + t.channel + begin * p.ldgy,
+                                      step * p.ldx, step * p.ldgy, count, p.lanes, t.there, [&](const auto& v, const auto& g, auto have) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) rw[i] = stat.y * w[i];
-    for (int64_t q = 0; q < count; q += BATCH) {
-        Values<T, E, STRIDED> v[BATCH], gv[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k)
-            if (q + k < count) {
-                v[k].load(x, p.lanes, t.there), x += dx;
-                if (GRAD) gv[k].load(gy, p.lanes, t.there), gy += dg;
+            for (int k = 0; k < batch_of<T, E, STRIDED, GRAD>(); ++k) {
+                const auto out = finished<T, E, STRIDED, GRAD, decltype(act)::value>(v[k], g[GRAD ? k : 0], w, b, stat, sums);
+                if (k < have) out.store(y, p.lanes, t.there), y += dy;
             }
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-            if (q + k >= count) break;
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float d = cbm::widen(v[k].v[i]) - stat.x;
-                const float z = d * rw[i] + b[i];
-                float out;
-                if constexpr (GRAD) {
-                    const float u = cbm::widen(gv[k].v[i]) * slope(z, p.act) * w[i];
-                    out = stat.y * (u - sums.x - d * stat.y * sums.y);
-                } else {
-                    out = activated(z, p.act);
-                }
-                v[k].v[i] = cbm::narrow<T>(out);
-            }
-            v[k].store(y, p.lanes, t.there), y += dy;
-        }
-    }
+        });
+    });
 }
 
 template <class T, int E, bool STRIDED>
@@ -374,18 +442,22 @@ constexpr int blocks_resident(int e, bool grad) { return e == 8 ? (grad ? 2 : 3)
 // A team to a tile: samples that lie in it are done with, of longer ones their part is left in `pieces`.
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kernel(const Params p) {
-    __shared__ float2 s_part[THREADS], s_stat[THREADS];
+    __shared__ float2 s_part[2][THREADS], s_stat[THREADS];  // (parts: of this sample and of the one before, which may still be read)
     __shared__ float2 s_channel[GRAD ? THREADS * E : 1];
     cbm::wait_before();
     const Team t(p, E, STRIDED);
     const int64_t tile = (int64_t)blockIdx.x * (THREADS / p.team) + t.id;
     if (tile >= p.tiles) return;
-    float2 *part = s_part + t.id * t.size, *stat = s_stat + t.id * t.size;
+    float2 *part = s_part[0] + t.id * t.size, *stat = s_stat + t.id * t.size;
     float w[E], b[E], gw[E], gb[E];
     fetch_params<T, E, STRIDED>(p, t, w, b);
 #pragma unroll
     for (int i = 0; i < E; ++i) gw[i] = gb[i] = 0.f;
-    const int64_t tb = tile_start(p, tile * p.tile), te = tile_start(p, (tile + 1) * p.tile);
+    int64_t s, after;
+    samples_at(p, tile * p.tile, (tile + 1) * p.tile, s, after);
+    const int64_t tb = tile_start(p, tile * p.tile, s), te = tile_start(p, (tile + 1) * p.tile, after);
+    if (p.longer && t.thread < 2 && blockIdx.y == 0) p.longer[t.thread * p.tiles + tile] = -1;
+    t.sync();
     const T *x = static_cast<const T*>(p.x) + t.channel, *gy = static_cast<const T*>(p.gy) + t.channel;
     using V = Values<T, E, STRIDED>;
     if (p.ptr && tb < te) {  // rows of no sample
@@ -397,50 +469,46 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
         for (int64_t row = tb + t.row_in; t.on() && row < min(te, head); row += t.at_once) none.store(y + row * p.ldy, p.lanes, t.there);
         for (int64_t row = max(tb, tail) + t.row_in; t.on() && row < te; row += t.at_once) none.store(y + row * p.ldy, p.lanes, t.there);
     }
-    int64_t s = tb < te ? max(sample_at(p, tb), (int64_t)0) : p.n_samples;
-    int64_t a = s < p.n_samples ? start_of(p, s) : te, e;
+    // (the sample at the tile's nominal start is the one at its start, too; where several start there, those before the last are empty)
+    s = tb < te ? max(s, (int64_t)0) : p.n_samples;
+    int64_t a = s < p.n_samples ? start_of(p, s) : te, next = s < p.n_samples ? start_of(p, s + 1) : te, e;
     for (; s < p.n_samples && a < te; ++s, a = e) {
-        e = start_of(p, s + 1);
+        e = next;
+        if (s + 1 < p.n_samples) next = start_of(p, s + 2);  // on its way meanwhile
         const int64_t lo = max(a, tb), hi = min(e, te);
         if (lo >= hi) continue;
-        const bool whole = e - a <= p.tile;
         const int rows = (int)(hi - lo);  // (at most two tiles, which fit 31 bits)
-        constexpr int BATCH = GRAD && E == 8 ? 2 : 4;
+        constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
         float2 at{0.f, 0.f};
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-        float mean[E], m2[E];  // of each channel; for the gradient the sums of g xh and g
+        float mean[E], m2[E];  // of each channel (also of missing ones, which are left out in the end); for the gradient the sums of g xh and g
         int n = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
         if (t.on()) {
-            const T *px = x + (lo + t.row_in) * p.ldx, *pg = gy + (lo + t.row_in) * p.ldgy;
-            const int64_t dx = t.at_once * p.ldx, dg = t.at_once * p.ldgy;
-            for (int left = (rows - t.row_in + t.at_once - 1) / t.at_once; left > 0; left -= BATCH) {
-                V v[BATCH], gv[BATCH];
-                const int have = min(BATCH, left);
+            auto rows_of = [&](auto&& f) {
+                for_rows<T, E, STRIDED, GRAD>(x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
+                                              (rows - t.row_in + t.at_once - 1) / t.at_once, p.lanes, t.there, f);
+            };
+            if constexpr (GRAD) {
+                with_activation(p.act, [&](auto act) {
+                    rows_of([&](const auto& v, const auto& gv, auto have) {
 #pragma unroll
-                for (int k = 0; k < BATCH; ++k)
-                    if (k < have) {
-                        v[k].load(px, p.lanes, t.there), px += dx;
-                        if (GRAD) gv[k].load(pg, p.lanes, t.there), pg += dg;
-                    }
-                if constexpr (GRAD) {
-#pragma unroll
-                    for (int k = 0; k < BATCH; ++k)
-                        if (k < have)
+                        for (int k = 0; k < BATCH; ++k)
 #pragma unroll
                             for (int i = 0; i < E; ++i) {
-                                if (!has<STRIDED>(i, t.there)) break;
                                 const float xh = (cbm::widen(v[k].v[i]) - at.x) * at.y;
-                                const float g = cbm::widen(gv[k].v[i]) * slope(xh * w[i] + b[i], p.act);
+                                const float g = k < have ? cbm::widen(gv[k].v[i]) * slope<decltype(act)::value>(xh * w[i] + b[i]) : 0.f;
                                 mean[i] += g * xh;
                                 m2[i] += g;
                             }
-                } else {
+                    });
+                });
+            } else {
+                rows_of([&](const auto& v, const auto&, auto have) {
                     const float share = 1.f / (float)have, to_mean = (float)have / (float)(n + have), to_squares = (float)n * to_mean;
 #pragma unroll
                     for (int i = 0; i < E; ++i) {
-                        if (!has<STRIDED>(i, t.there)) break;
                         float sum = 0.f, squares = 0.f;
 #pragma unroll
                         for (int k = 0; k < BATCH; ++k) sum += k < have ? cbm::widen(v[k].v[i]) : 0.f;
@@ -455,7 +523,7 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
                         m2[i] += squares + d * d * to_squares;
                     }
                     n += have;
-                }
+                });
             }
             float2 mine{0.f, 0.f};
             if constexpr (GRAD) {
@@ -478,27 +546,41 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
             part[t.thread] = mine;
         }
         t.sync();
-        join_groups<!GRAD, E, STRIDED>(p, t, part, rows, [&](int g, float2 all) {
+        const float share = 1.f / ((float)rows * (float)p.width);
+        const bool whole = e - a <= p.tile;
+        // for a group: what was found, from its threads' joined parts
+        auto finish = [&](int group, float2 all, bool writes) {
             if (!whole) {
                 const int64_t slot = a > tile * p.tile ? 1 : 0;  // a longer sample that starts inside the tile is its second one
-                p.pieces[(slot * p.groups + t.group0 + g) * p.tiles + tile] = all;
-                return;
+                if (writes) p.pieces[(slot * p.groups + group) * p.tiles + tile] = all;
+                return all;
             }
-            const float share = 1.f / ((float)rows * (float)p.width);
-            if constexpr (GRAD) {
-                stat[g] = float2{all.x * share, all.y * share};
-            } else {
-                const float r = rsqrtf(all.y * share + p.eps);
-                stat[g] = float2{all.x, r};
-                if (p.mean) {
-                    p.mean[s * p.groups + t.group0 + g] = all.x;
-                    p.r[s * p.groups + t.group0 + g] = r;
-                }
+            if constexpr (GRAD) return float2{all.x * share, all.y * share};
+            const float2 found{all.x, rsqrtf(all.y * share + p.eps)};
+            if (writes && p.mean) {
+                p.mean[s * p.groups + group] = found.x;
+                p.r[s * p.groups + group] = found.y;
             }
-        });
-        t.sync();
-        if (!whole) continue;
-        const float2 found = stat[t.group - t.group0];
+            return found;
+        };
+        float2 found{0.f, 0.f};
+        if (p.lanes * t.at_once <= FEW) {
+            const Join<!GRAD, E, STRIDED> join{p, t, part + (t.group - t.group0) * p.lanes, rows};
+            found = finish(t.group, join.template run<false>(), t.row_in == 0 && t.lane == 0);
+            part = part == s_part[0] + t.id * t.size ? s_part[1] + t.id * t.size : s_part[0] + t.id * t.size;
+        } else {
+            for (int g = t.thread >> 5; g < t.groups; g += t.size >> 5) {
+                const Join<!GRAD, E, STRIDED> join{p, t, part + g * p.lanes, rows};
+                const float2 one = finish(t.group0 + g, join.template run<true>(), (t.thread & 31) == 0);
+                if ((t.thread & 31) == 0) stat[g] = one;
+            }
+            t.sync();
+            found = stat[t.group - t.group0];
+        }
+        if (!whole) {
+            if (t.thread == 0 && blockIdx.y == 0) p.longer[(a > tile * p.tile ? p.tiles : 0) + tile] = s;
+            continue;
+        }
         write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, hi, w, b, GRAD ? at : found, found);
     }
     if constexpr (GRAD) {
@@ -521,47 +603,64 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
     }
 }
 
-// The pieces of each sample that is longer than a tile, by the block of the tile in which it starts, a warp to a group.  The blocks behind
-// those of the tiles add up the channels' sums, 32 each.
+// The pieces of each sample that is longer than a tile, JOINERS threads to a group.  Block x: a tile, for the sample that starts in it, or
+// where samples are equal, a sample; y: the groups y, y + gridDim.y, ...  The blocks behind add up the channels' sums, 32 each.
+constexpr int JOINERS = 256;
+
+__device__ __forceinline__ float joiners_sum(float v, float* s_sum) {
+    v = lanes_sum(v, 32);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < JOINERS / 32; ++i) v += s_sum[i];
+    return v;
+}
+
 template <class T, bool GRAD>
-__global__ void __launch_bounds__(1024) join_kernel(const Params p, int64_t tiles) {
+__global__ void __launch_bounds__(JOINERS) join_kernel(const Params p, const int64_t starts) {
+    __shared__ float s_sum[JOINERS / 32];
     cbm::wait_before();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (blockIdx.x < tiles) {
-        const int64_t tile = blockIdx.x, end = (tile + 1) * p.tile;
-        if (end > p.n_rows) return;
-        const int64_t s = sample_at(p, end - 1);
-        if (s < 0 || s >= p.n_samples) return;
+    if (blockIdx.x < starts) {
+        int64_t s = blockIdx.x, tile = blockIdx.x;
+        if (p.ptr) {
+            // (a sample that starts with the tile fills it)
+            s = p.longer[p.tiles + tile];
+            if (s < 0) s = p.longer[tile];
+            if (s < 0 || start_of(p, s) < tile * p.tile) return;
+        }
         const int64_t a = start_of(p, s), e = start_of(p, s + 1);
-        if (a < tile * p.tile || e - a <= p.tile) return;
+        tile = a / p.tile;
         const int64_t last = (e - 1) / p.tile;
         const float count = (float)(e - a) * (float)p.width;
-        for (int g = warp; g < p.groups; g += 32) {
+        for (int g = blockIdx.y; g < p.groups; g += gridDim.y) {
             const float2* found = p.pieces + (int64_t)g * p.tiles;
             // of the first tile it is the second piece unless the sample starts with the tile
             auto piece = [&](int64_t q) { return found[(q == tile && a > tile * p.tile ? p.groups * p.tiles : 0) + q]; };
             if constexpr (GRAD) {
                 float2 all{0.f, 0.f};
-                for (int64_t q = tile + lane; q <= last; q += 32) {
+#pragma unroll 4
+                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) {
                     const float2 one = piece(q);
                     all.x += one.x, all.y += one.y;
                 }
-                all.x = lanes_sum(all.x, 32), all.y = lanes_sum(all.y, 32);
-                if (lane == 0) p.joined[tile * p.groups + g] = float2{all.x / count, all.y / count};
+                all = float2{joiners_sum(all.x, s_sum), joiners_sum(all.y, s_sum)};
+                if (threadIdx.x == 0) p.joined[tile * p.groups + g] = float2{all.x / count, all.y / count};
             } else {
                 auto rows = [&](int64_t q) { return (float)(min(e, (q + 1) * p.tile) - max(a, q * p.tile)); };
                 const float ref = piece(tile).x;
                 float m = 0.f, squares = 0.f;
 #pragma unroll 4
-                for (int64_t q = tile + lane; q <= last; q += 32) m += rows(q) * (piece(q).x - ref);
-                const float mean = ref + lanes_sum(m, 32) / (float)(e - a);
+                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) m += rows(q) * (piece(q).x - ref);
+                const float mean = ref + joiners_sum(m, s_sum) / (float)(e - a);
 #pragma unroll 4
-                for (int64_t q = tile + lane; q <= last; q += 32) {
+                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) {
                     const float2 one = piece(q);
                     squares += one.y + rows(q) * (float)p.width * (one.x - mean) * (one.x - mean);
                 }
-                const float r = rsqrtf(lanes_sum(squares, 32) / count + p.eps);
-                if (lane == 0) {
+                const float r = rsqrtf(joiners_sum(squares, s_sum) / count + p.eps);
+                if (threadIdx.x == 0) {
                     p.joined[tile * p.groups + g] = float2{mean, r};
                     if (p.mean) {
                         p.mean[s * p.groups + g] = mean;
@@ -571,23 +670,22 @@ __global__ void __launch_bounds__(1024) join_kernel(const Params p, int64_t tile
             }
         }
     } else if constexpr (GRAD) {
-        __shared__ float2 s_sum[32][33];
-        const int c = (int)(blockIdx.x - tiles) * 32 + lane;
+        if (blockIdx.y) return;
+        __shared__ float2 s_part[JOINERS / 32][33];
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (int)(blockIdx.x - starts) * 32 + lane;
         float2 all{0.f, 0.f};
         if (c < p.c)
-#pragma unroll 4
-            for (int64_t q = warp; q < p.parts; q += 32) {
+#pragma unroll 8
+            for (int64_t q = warp; q < p.parts; q += JOINERS / 32) {
                 const float2 one = p.channels[q * p.c + c];
                 all.x += one.x, all.y += one.y;
             }
-        s_sum[warp][lane] = all;
+        s_part[warp][lane] = all;
         __syncthreads();
-        all = s_sum[lane][warp];
-        all.x = lanes_sum(all.x, 32), all.y = lanes_sum(all.y, 32);
-        const int mine = (int)(blockIdx.x - tiles) * 32 + warp;
-        if (lane == 0 && mine < p.c) {
-            if (p.gw) p.gw[mine] = all.x;
-            if (p.gb) p.gb[mine] = all.y;
+        if (warp == 0 && c < p.c) {
+            for (int i = 1; i < JOINERS / 32; ++i) all.x += s_part[i][lane].x, all.y += s_part[i][lane].y;
+            if (p.gw) p.gw[c] = all.x;
+            if (p.gb) p.gb[c] = all.y;
         }
     }
 }
@@ -602,13 +700,10 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) long_kernel
     float w[E], b[E];
     fetch_params<T, E, STRIDED>(p, t, w, b);
     const int64_t begin = tile * p.tile, end = min(begin + p.tile, p.n_rows);
-    int64_t last = -1;
-    for (int k = 0; k < 2; ++k) {
-        const int64_t s = sample_at(p, k == 0 ? end - 1 : begin);
-        if (s < 0 || s >= p.n_samples || s == last) continue;
-        last = s;
+    for (int k = 1; k >= 0; --k) {
+        const int64_t s = p.longer[k * p.tiles + tile];
+        if (s < 0) continue;
         const int64_t a = start_of(p, s), e = start_of(p, s + 1);
-        if (e - a <= p.tile || !t.on()) continue;
         const int64_t lo = max(a, begin), hi = min(e, end);
         const float2 found = p.joined[(a / p.tile) * p.groups + t.group];
         float2 at = found;
@@ -627,6 +722,12 @@ __device__ __forceinline__ float block_sum(float v) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) s += part[i];
+    return s;
+}
+
+__device__ __forceinline__ float slope_by(float z, int act) {
+    float s;
+    with_activation(act, [&](auto a) { s = slope<decltype(a)::value>(z); });
     return s;
 }
 
@@ -653,14 +754,14 @@ __global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
         if constexpr (!GRAD) {
             each([&](int64_t row, int c, float v) {
                 const float z = (v - mean) * (r * param<T>(p.w, p.wide_params, c, 1.f)) + param<T>(p.b, p.wide_params, c, 0.f);
-                static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(activated(z, p.act));
+                with_activation(p.act, [&](auto act) { static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(activated<decltype(act)::value>(z)); });
             });
             if (threadIdx.x == 0 && p.mean) p.mean[unit] = mean, p.r[unit] = r;
         } else {
             float su = 0.f, sux = 0.f;
             auto u_of = [&](int64_t row, int c, float xh) {
                 const float w = param<T>(p.w, p.wide_params, c, 1.f);
-                return cbm::widen(gy[row * p.ldgy + c]) * slope(xh * w + param<T>(p.b, p.wide_params, c, 0.f), p.act) * w;
+                return cbm::widen(gy[row * p.ldgy + c]) * slope_by(xh * w + param<T>(p.b, p.wide_params, c, 0.f), p.act) * w;
             };
             each([&](int64_t row, int c, float v) {
                 const float xh = (v - mean) * r, u = u_of(row, c, xh);
@@ -690,7 +791,7 @@ __global__ void __launch_bounds__(THREADS) wide_params_kernel(const Params p) {
         const int64_t last = start_of(p, s + 1);
         for (int64_t row = start_of(p, s); row < last; ++row) {
             const float xh = (cbm::widen(static_cast<const T*>(p.x)[row * p.ldx + c]) - at.x) * at.y;
-            const float g = cbm::widen(static_cast<const T*>(p.gy)[row * p.ldgy + c]) * slope(xh * w + b, p.act);
+            const float g = cbm::widen(static_cast<const T*>(p.gy)[row * p.ldgy + c]) * slope_by(xh * w + b, p.act);
             all.x += g * xh, all.y += g;
         }
     }
@@ -768,8 +869,9 @@ struct Plan {
         }
         way = TILES;
         slab_groups = THREADS / lanes < groups ? THREADS / lanes : groups;
-        // Four rows of a slab at once, at least a warp.
-        for (team = 32; team < THREADS && team < 4 * slab_groups * lanes;) team *= 2;
+        // Four rows at once, or where samples are short one, so that more of them are under way.
+        const int wanted = (n_samples && n_rows / n_samples > 64 ? 4 : 1) * slab_groups * lanes;
+        for (team = 32; team < THREADS && team < wanted;) team *= 2;
         const int at_once = team / (slab_groups * lanes), slabs = (groups + slab_groups - 1) / slab_groups;
         int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
         if (teams < 1) teams = 1;
@@ -780,7 +882,7 @@ struct Plan {
         joins = ptr || rows_each > tile;
     }
     int threads() const { return (rows.slots * rows.at_once + 31) / 32 * 32; }
-    int64_t piece_bytes(int groups) const { return way == TILES && joins ? 8 * 3 * tiles * groups : 0; }
+    int64_t piece_bytes(int groups) const { return way == TILES && joins ? 8 * (3 * tiles * groups + 2 * tiles) : 0; }
     int64_t bytes(int64_t n_samples, int c, int groups, bool grad) const {
         return (grad ? 8 * parts * c : 0) + piece_bytes(groups) + (way == WIDE && grad ? 8 * n_samples * groups : 0);
     }
@@ -832,6 +934,7 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
     } else if (plan.way == TILES) {
         p.pieces = reinterpret_cast<float2*>(workspace);
         p.joined = p.pieces + 2 * p.tiles * p.groups;
+        if (plan.joins) p.longer = reinterpret_cast<int64_t*>(p.joined + p.tiles * p.groups);
         const int per_block = THREADS / p.team;
         const dim3 grid((unsigned)((p.tiles + per_block - 1) / per_block), (p.groups + p.slab_groups - 1) / p.slab_groups);
         with_form<T>(plan.form, [&](auto e, auto strided) {
@@ -839,8 +942,9 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
             constexpr bool STRIDED = decltype(strided)::value;
             cbm::launch_next(tiles_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
             if (!plan.joins) return;
-            joins = p.tiles;
-            cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)(joins + (sums ? (p.c + 31) / 32 : 0))), 1024, 0, on, p, joins);
+            joins = p.ptr ? p.tiles : p.n_samples;
+            const int across = p.ptr ? (p.groups < 4 ? p.groups : 4) : p.groups;  // (most blocks of tiles find nothing to do)
+            cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)(joins + (sums ? (p.c + 31) / 32 : 0)), across), JOINERS, 0, on, p, joins);
             cbm::launch_next(long_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
         });
     } else {
@@ -849,7 +953,7 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
         if (p.ptr) cbm::launch_next(outside_kernel<T>, blocks_for(p.n_rows), THREADS, 0, on, p);
         if (sums) cbm::launch_next(wide_params_kernel<T>, dim3((unsigned)p.parts, (p.c + THREADS - 1) / THREADS), THREADS, 0, on, p);
     }
-    if (sums && !joins) cbm::launch_next(join_kernel<T, true>, dim3((p.c + 31) / 32), 1024, 0, on, p, joins);
+    if (sums && !joins) cbm::launch_next(join_kernel<T, true>, dim3((p.c + 31) / 32), JOINERS, 0, on, p, joins);
 }
 
 // Workspace of a call, whatever the type and the alignment of its rows.
