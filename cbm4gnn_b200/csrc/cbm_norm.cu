@@ -128,21 +128,23 @@ struct RowShape {
 };
 
 // Sums of two values over a group's threads.
-__device__ __forceinline__ float2 group_sum(float2 v, const RowShape& h, float2* s_warp) {
+// (`s_warp` is another place from one sum to the next, so that a barrier for each does.)
+__device__ __forceinline__ float2 group_sum(float2 v, const RowShape& h, float2 (*s_warp)[32], int& turn) {
     if (!h.warps) return float2{lanes_sum(v.x, 1 << h.shift), lanes_sum(v.y, 1 << h.shift)};
     v = float2{lanes_sum(v.x, 32), lanes_sum(v.y, 32)};
     const int warp = threadIdx.x >> 5, first = warp / h.warps * h.warps;
+    float2* const here = s_warp[turn ^= 1];
+    if ((threadIdx.x & 31) == 0) here[warp] = v;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_warp[warp] = v;
-    __syncthreads();
-    v = s_warp[first];
-    for (int i = 1; i < h.warps; ++i) v.x += s_warp[first + i].x, v.y += s_warp[first + i].y;
+    v = here[first];
+    for (int i = 1; i < h.warps; ++i) v.x += here[first + i].x, v.y += here[first + i].y;
     return v;
 }
 
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowShape h) {
-    __shared__ float2 s_warp[32];
+    __shared__ float2 s_warp[2][32];
+    int turn = 0;
     cbm::wait_before();
     const int row_in = threadIdx.x / h.slots, slot = threadIdx.x % h.slots, lane = slot % h.padded();
     const int group = blockIdx.y * p.slab_groups + slot / h.padded();
@@ -180,14 +182,14 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowSha
             s.x += x[i];
         }
         fetch(row + step);  // on its way meanwhile
-        const float mean = group_sum(s, h, s_warp).x * share;
+        const float mean = group_sum(s, h, s_warp, turn).x * share;
         s.x = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] = i < now ? x[i] - mean : 0.f;
             s.x += x[i] * x[i];
         }
-        const float r = rsqrtf(group_sum(s, h, s_warp).x * share + p.eps);
+        const float r = rsqrtf(group_sum(s, h, s_warp, turn).x * share + p.eps);
         V out;
         if constexpr (!GRAD) {
             with_activation(p.act, [&](auto act) {
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowSha
                     s.y += u[i] * x[i];
                 }
             });
-            s = group_sum(s, h, s_warp);
+            s = group_sum(s, h, s_warp, turn);
 #pragma unroll
             for (int i = 0; i < E; ++i) out.v[i] = cbm::narrow<T>(r * (u[i] - s.x * share - x[i] * (s.y * share)));
         }
@@ -328,6 +330,7 @@ struct Join {
     template <bool WARP>
     __device__ __forceinline__ float2 run() const {
         float2 s{0.f, 0.f};
+        if (rows == 0) return s;
         auto each = [&](auto&& f) {
             if constexpr (WARP) together(f);
             else alone(f);
@@ -439,6 +442,97 @@ __device__ __forceinline__ void fetch_params(const Params& p, const Team& t, flo
 // Blocks of an SM: what their registers leave room for without spilling.
 constexpr int blocks_resident(int e, bool grad) { return e == 8 ? (grad ? 2 : 3) : e == 4 && grad ? 3 : 4; }
 
+// What a thread finds in `rows` rows of a sample from row lo on: the mean over its values and the squares around it; or, for the gradient,
+// its sums of u and u xh, and by channel those of g xh and g, added to gw and gb.
+template <class T, int E, bool STRIDED, bool GRAD>
+__device__ __forceinline__ float2 gathered(const Params& p, const Team& t, int64_t lo, int rows, const float (&w)[E], const float (&b)[E], float2 at,
+                                           float (&gw)[E], float (&gb)[E]) {
+    constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
+    const T *x = static_cast<const T*>(p.x) + t.channel, *gy = static_cast<const T*>(p.gy) + t.channel;
+    float2 mine{0.f, 0.f};
+    if (!t.on()) return mine;
+    float mean[E], m2[E];  // of each channel (also of missing ones, which are left out in the end); for the gradient the sums of g xh and g
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
+    auto rows_of = [&](auto&& f) {
+        for_rows<T, E, STRIDED, GRAD>(x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
+                                      (rows - t.row_in + t.at_once - 1) / t.at_once, p.lanes, t.there, f);
+    };
+    if constexpr (GRAD) {
+        with_activation(p.act, [&](auto act) {
+            rows_of([&](const auto& v, const auto& gv, auto have) {
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float xh = (cbm::widen(v[k].v[i]) - at.x) * at.y;
+                        const float g = k < have ? cbm::widen(gv[k].v[i]) * slope<decltype(act)::value>(xh * w[i] + b[i]) : 0.f;
+                        mean[i] += g * xh;
+                        m2[i] += g;
+                    }
+            });
+        });
+    } else {
+        rows_of([&](const auto& v, const auto&, auto have) {
+            const float share = 1.f / (float)have, to_mean = (float)have / (float)(n + have), to_squares = (float)n * to_mean;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                float sum = 0.f, squares = 0.f;
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) sum += k < have ? cbm::widen(v[k].v[i]) : 0.f;
+                const float here = sum * share;
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const float d = k < have ? cbm::widen(v[k].v[i]) - here : 0.f;
+                    squares += d * d;
+                }
+                const float d = here - mean[i];
+                mean[i] += d * to_mean;
+                m2[i] += squares + d * d * to_squares;
+            }
+            n += have;
+        });
+    }
+    if constexpr (GRAD) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            mine.x += m2[i] * w[i];    // u
+            mine.y += mean[i] * w[i];  // u xh
+            gw[i] += mean[i];
+            gb[i] += m2[i];
+        }
+    } else {
+        float shift = 0.f;
+#pragma unroll
+        for (int i = 1; i < E; ++i) shift += has<STRIDED>(i, t.there) ? mean[i] - mean[0] : 0.f;
+        mine.x = mean[0] + shift / (float)t.there;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (has<STRIDED>(i, t.there)) mine.y += m2[i] + (float)n * (mean[i] - mine.x) * (mean[i] - mine.x);
+    }
+    return mine;
+}
+
+// A team's sums of g xh and g, as part `to`.
+template <class T, int E, bool STRIDED>
+__device__ __forceinline__ void store_channels(const Params& p, const Team& t, const float (&gw)[E], const float (&gb)[E], float2* s_channel, int64_t to) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_channel[i * t.size + t.thread] = float2{gw[i], gb[i]};
+    t.sync();
+    if (t.row_in) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!has<STRIDED>(i, t.there)) break;
+        float2 all = s_channel[i * t.size + t.thread];
+        for (int q = 1; q < t.at_once; ++q) {
+            const float2 one = s_channel[i * t.size + t.thread + q * t.vectors];
+            all.x += one.x, all.y += one.y;
+        }
+        p.channels[to * p.c + t.channel + i * (STRIDED ? p.lanes : 1)] = all;
+    }
+}
+
 // A team to a tile: samples that lie in it are done with, of longer ones their part is left in `pieces`.
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kernel(const Params p) {
@@ -458,11 +552,9 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
     const int64_t tb = tile_start(p, tile * p.tile, s), te = tile_start(p, (tile + 1) * p.tile, after);
     if (p.longer && t.thread < 2 && blockIdx.y == 0) p.longer[t.thread * p.tiles + tile] = -1;
     t.sync();
-    const T *x = static_cast<const T*>(p.x) + t.channel, *gy = static_cast<const T*>(p.gy) + t.channel;
-    using V = Values<T, E, STRIDED>;
     if (p.ptr && tb < te) {  // rows of no sample
         const int64_t head = p.n_samples ? start_of(p, 0) : p.n_rows, tail = p.n_samples ? start_of(p, p.n_samples) : p.n_rows;
-        V none;
+        Values<T, E, STRIDED> none;
 #pragma unroll
         for (int i = 0; i < E; ++i) none.v[i] = cbm::narrow<T>(0.f);
         T* y = static_cast<T*>(p.y) + t.channel;
@@ -478,73 +570,9 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
         const int64_t lo = max(a, tb), hi = min(e, te);
         if (lo >= hi) continue;
         const int rows = (int)(hi - lo);  // (at most two tiles, which fit 31 bits)
-        constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
         float2 at{0.f, 0.f};
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-        float mean[E], m2[E];  // of each channel (also of missing ones, which are left out in the end); for the gradient the sums of g xh and g
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
-        if (t.on()) {
-            auto rows_of = [&](auto&& f) {
-                for_rows<T, E, STRIDED, GRAD>(x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
-                                              (rows - t.row_in + t.at_once - 1) / t.at_once, p.lanes, t.there, f);
-            };
-            if constexpr (GRAD) {
-                with_activation(p.act, [&](auto act) {
-                    rows_of([&](const auto& v, const auto& gv, auto have) {
-#pragma unroll
-                        for (int k = 0; k < BATCH; ++k)
-#pragma unroll
-                            for (int i = 0; i < E; ++i) {
-                                const float xh = (cbm::widen(v[k].v[i]) - at.x) * at.y;
-                                const float g = k < have ? cbm::widen(gv[k].v[i]) * slope<decltype(act)::value>(xh * w[i] + b[i]) : 0.f;
-                                mean[i] += g * xh;
-                                m2[i] += g;
-                            }
-                    });
-                });
-            } else {
-                rows_of([&](const auto& v, const auto&, auto have) {
-                    const float share = 1.f / (float)have, to_mean = (float)have / (float)(n + have), to_squares = (float)n * to_mean;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        float sum = 0.f, squares = 0.f;
-#pragma unroll
-                        for (int k = 0; k < BATCH; ++k) sum += k < have ? cbm::widen(v[k].v[i]) : 0.f;
-                        const float here = sum * share;
-#pragma unroll
-                        for (int k = 0; k < BATCH; ++k) {
-                            const float d = k < have ? cbm::widen(v[k].v[i]) - here : 0.f;
-                            squares += d * d;
-                        }
-                        const float d = here - mean[i];
-                        mean[i] += d * to_mean;
-                        m2[i] += squares + d * d * to_squares;
-                    }
-                    n += have;
-                });
-            }
-            float2 mine{0.f, 0.f};
-            if constexpr (GRAD) {
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    mine.x += m2[i] * w[i];    // u
-                    mine.y += mean[i] * w[i];  // u xh
-                    gw[i] += mean[i];
-                    gb[i] += m2[i];
-                }
-            } else {
-                float shift = 0.f;
-#pragma unroll
-                for (int i = 1; i < E; ++i) shift += has<STRIDED>(i, t.there) ? mean[i] - mean[0] : 0.f;
-                mine.x = mean[0] + shift / (float)t.there;
-#pragma unroll
-                for (int i = 0; i < E; ++i)
-                    if (has<STRIDED>(i, t.there)) mine.y += m2[i] + (float)n * (mean[i] - mine.x) * (mean[i] - mine.x);
-            }
-            part[t.thread] = mine;
-        }
+        part[t.thread] = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
         t.sync();
         const float share = 1.f / ((float)rows * (float)p.width);
         const bool whole = e - a <= p.tile;
@@ -584,22 +612,7 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
         write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, hi, w, b, GRAD ? at : found, found);
     }
     if constexpr (GRAD) {
-        if (!p.channels) return;
-        float2* mine = s_channel + (t.id * t.size) * E;
-#pragma unroll
-        for (int i = 0; i < E; ++i) mine[i * t.size + t.thread] = float2{gw[i], gb[i]};
-        t.sync();
-        if (t.row_in == 0)
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                if (!has<STRIDED>(i, t.there)) break;
-                float2 all = mine[i * t.size + t.thread];
-                for (int q = 1; q < t.at_once; ++q) {
-                    const float2 one = mine[i * t.size + t.thread + q * t.vectors];
-                    all.x += one.x, all.y += one.y;
-                }
-                p.channels[tile * p.c + t.channel + i * (STRIDED ? p.lanes : 1)] = all;
-            }
+        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, s_channel + t.id * t.size * E, tile);
     }
 }
 
@@ -709,6 +722,74 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) long_kernel
         float2 at = found;
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
         if (lo < hi) write_rows<T, E, STRIDED, GRAD, true>(p, t, lo, hi, w, b, at, found);
+    }
+}
+
+// ---- a few samples that are not long: a cluster of blocks to each ----------------------------------
+constexpr int CLUSTER = 8;
+
+// Every block has a stretch of the sample's rows; what it finds goes to all blocks of the cluster, which read their rows again, out of L1 or
+// L2: one launch, where tiles, joins and rows take three.  y: a slab of groups.
+template <class T, int E, bool STRIDED, bool GRAD>
+__global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) cluster_kernel(const Params p) {
+    __shared__ float2 s_part[THREADS], s_stat[THREADS], s_all[CLUSTER][THREADS];
+    __shared__ float2 s_channel[GRAD ? THREADS * E : 1];
+    u32 rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // the others' shared memory is there once all have started
+    cbm::wait_before();
+    const Team t(p, E, STRIDED);
+    const int64_t s = blockIdx.x / CLUSTER, each = (p.rows_each + CLUSTER - 1) / CLUSTER;
+    auto rows_of = [&](int64_t k) { return (int)max(min(p.rows_each - k * each, each), (int64_t)0); };
+    const int64_t lo = s * p.rows_each + min(rank * each, p.rows_each);
+    const int rows = rows_of(rank);
+    float w[E], b[E], gw[E], gb[E];
+    fetch_params<T, E, STRIDED>(p, t, w, b);
+#pragma unroll
+    for (int i = 0; i < E; ++i) gw[i] = gb[i] = 0.f;
+    float2 at{0.f, 0.f};
+    if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
+    s_part[t.thread] = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
+    __syncthreads();
+    for (int g = t.thread >> 5; g < t.groups; g += THREADS / 32) {
+        const Join<!GRAD, E, STRIDED> join{p, t, s_part + g * p.lanes, rows};
+        const float2 one = join.template run<true>();
+        if ((t.thread & 31) == 0) s_stat[g] = one;
+    }
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    for (int i = t.thread; i < t.groups * CLUSTER; i += THREADS) {
+        const int to = i / t.groups, g = i - to * t.groups;
+        u32 place;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(place) : "r"((u32)__cvta_generic_to_shared(&s_all[rank][g])), "r"(to));
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(place), "f"(s_stat[g].x), "f"(s_stat[g].y) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    const int mine = t.group - t.group0;
+    const float share = 1.f / ((float)p.rows_each * (float)p.width);
+    float2 found{0.f, 0.f};
+    if constexpr (GRAD) {
+        for (int k = 0; k < CLUSTER; ++k) found.x += s_all[k][mine].x, found.y += s_all[k][mine].y;
+        found = float2{found.x * share, found.y * share};
+    } else {
+        const float ref = s_all[0][mine].x;
+        float m = 0.f, squares = 0.f;
+        for (int k = 0; k < CLUSTER; ++k) m += (float)rows_of(k) * (s_all[k][mine].x - ref);
+        const float mean = ref + m / (float)p.rows_each;
+        for (int k = 0; k < CLUSTER; ++k) {
+            const float2 one = s_all[k][mine];
+            squares += one.y + (float)rows_of(k) * (float)p.width * (one.x - mean) * (one.x - mean);
+        }
+        found = float2{mean, rsqrtf(squares * share + p.eps)};
+        if (rank == 0 && p.mean && t.row_in == 0 && t.lane == 0) {
+            p.mean[s * p.groups + t.group] = found.x;
+            p.r[s * p.groups + t.group] = found.y;
+        }
+    }
+    write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, lo + rows, w, b, GRAD ? at : found, found);
+    if constexpr (GRAD) {
+        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, s_channel, blockIdx.x);
     }
 }
 
@@ -823,7 +904,7 @@ int check(const char* who, const Params& p, int32_t type) {
     return fits ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes, type or activation");
 }
 
-enum Way { ROWS, TILES, WIDE };
+enum Way { ROWS, TILES, CLUSTERS, WIDE };
 
 // The values of a row that fall to a thread: E of them, as one vector or (strided) as many threads of a group apart.
 struct Form {
@@ -869,10 +950,18 @@ struct Plan {
         }
         way = TILES;
         slab_groups = THREADS / lanes < groups ? THREADS / lanes : groups;
+        // A few samples whose rows a cluster goes over in some dozen turns: 1 000 x 64 9 us, 15 with tiles, joins and rows by themselves.
+        const int64_t slabs = (groups + slab_groups - 1) / slab_groups, turn = (int64_t)CLUSTER * (THREADS / (slab_groups * lanes));
+        if (!ptr && rows_each > 1 && n_samples * CLUSTER * slabs <= 2 * SMS && rows_each <= 48 * turn) {
+            way = CLUSTERS;
+            team = THREADS;
+            parts = n_samples * CLUSTER;
+            return;
+        }
         // Four rows at once, or where samples are short one, so that more of them are under way.
         const int wanted = (n_samples && n_rows / n_samples > 64 ? 4 : 1) * slab_groups * lanes;
         for (team = 32; team < THREADS && team < wanted;) team *= 2;
-        const int at_once = team / (slab_groups * lanes), slabs = (groups + slab_groups - 1) / slab_groups;
+        const int at_once = team / (slab_groups * lanes);
         int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
         if (teams < 1) teams = 1;
         tile = (n_rows + teams - 1) / teams;
@@ -930,6 +1019,22 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
             const unsigned threads = plan.threads();
             const dim3 grid((unsigned)plan.blocks, (p.groups + p.slab_groups - 1) / p.slab_groups);
             cbm::launch_next(rows_kernel<T, decltype(e)::value, decltype(strided)::value, GRAD>, grid, threads, sums ? 8 * threads : 0, on, p, plan.rows);
+        });
+    } else if (plan.way == CLUSTERS) {
+        with_form<T>(plan.form, [&](auto e, auto strided) {
+            cudaLaunchAttribute attrs[2] = {};
+            attrs[0].id = cudaLaunchAttributeClusterDimension;
+            attrs[0].val.clusterDim.x = CLUSTER;
+            attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+            attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attrs[1].val.programmaticStreamSerializationAllowed = 1;
+            cudaLaunchConfig_t config = {};
+            config.gridDim = dim3((unsigned)plan.parts, (p.groups + p.slab_groups - 1) / p.slab_groups);
+            config.blockDim = dim3(THREADS);
+            config.stream = on.s;
+            config.attrs = attrs;
+            config.numAttrs = on.captured ? 1 : 2;
+            (void)cudaLaunchKernelEx(&config, cluster_kernel<T, decltype(e)::value, decltype(strided)::value, GRAD>, static_cast<Params>(p));
         });
     } else if (plan.way == TILES) {
         p.pieces = reinterpret_cast<float2*>(workspace);
@@ -1009,7 +1114,7 @@ extern "C" int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* 
     if (ldgy < channels) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: rows of the gradient overlap");
     if (n_rows && (!x || !gy || !gx)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
     const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), true);
-    if (n_rows && plan.way == TILES && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
+    if (n_rows && (plan.way == TILES || plan.way == CLUSTERS) && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
     const int64_t need = plan.bytes(n_samples, channels, groups, true);
     if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: workspace too small");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));

@@ -409,4 +409,11 @@ def test_a_normed_model_by_itself_is_one_graph():
         y = model(x, ei)
         h = group_norm(model.layers[0](x, ei), 8, activation="relu")
         assert torch.equal(y, model.layers[1](h, ei))
-        assert torch.equal(y, model(x, ei, ptr=torch.tensor([0, c.num_rows], device="cuda")))
+        # given as a list of one graph it goes another way, whose sums are ordered otherwise: each is within its bound of the same values
+        first = model.layers[0](x, ei)
+        ptr = torch.tensor([0, c.num_rows], device="cuda")
+        listed = group_norm(first, 8, activation="relu", ptr=ptr)
+        for got in (h, listed):
+            want, bound = norm64(first, 8, None, None, [0, c.num_rows], 1e-5, "relu", y=got)
+            assert_within(got, want["y"], bound["y"])
+        assert torch.equal(model(x, ei, ptr=ptr), model.layers[1](listed, ei))
