@@ -894,39 +894,29 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         }
         if (active > 1) {
             cluster_barrier();
-            // this block's rows of the sum, for all, a thread eight columns of a row
-            const int rows = (m + active - 1) / active, c = 8 * (threadIdx.x & 15), last = rank < active ? min(rows * rank + rows, m) : 0;
-            for (int r = rows * rank + (int)(threadIdx.x >> 4); r < last; r += SMALL_THREADS / 16) {
-                float v[8];
+            // This block's rows of the sum, for all, a warp to a row: what its lanes read and write in another block is contiguous (eight
+            // values to a lane, whose two fetches leave gaps, took 5 600 cycles, one for each 16 bytes).
+            const int rows = (m + active - 1) / active, c = 4 * lane, last = rank < active ? min(rows * rank + rows, m) : 0;
+            for (int r = rows * rank + warp; r < last; r += SMALL_THREADS / 32) {
+                // (all parts on their way together; in place of one that there is none of, this block's own, which is not added)
+                const u32 at = smem_u32(&at_sum(r, c));
+                float4 x[SMALL_BLOCKS];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = 0.f;
-                const u32 lo = smem_u32(&at_sum(r, c)), hi = smem_u32(&at_sum(r, c + 4));
-                for (int i0 = 0; i0 < active; i0 += 4) {  // (four blocks' parts on their way together; the last one's again for those that are not there)
-                    float4 x[4], y[4];
+                for (int i = 0; i < SMALL_BLOCKS; ++i)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
+                                 : "r"(in_block(at, i < active ? i : rank)));
+                float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int from_block = min(i0 + i, active - 1);
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(x[i].x), "=f"(x[i].y), "=f"(x[i].z), "=f"(x[i].w)
-                                     : "r"(in_block(lo, from_block)));
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(y[i].x), "=f"(y[i].y), "=f"(y[i].z), "=f"(y[i].w)
-                                     : "r"(in_block(hi, from_block)));
-                    }
+                for (int i = 0; i < SMALL_BLOCKS; ++i)
+                    if (i < active) v[0] += x[i].x, v[1] += x[i].y, v[2] += x[i].z, v[3] += x[i].w;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i0 + i < active) {
-                            v[0] += x[i].x, v[1] += x[i].y, v[2] += x[i].z, v[3] += x[i].w;
-                            v[4] += y[i].x, v[5] += y[i].y, v[6] += y[i].z, v[7] += y[i].w;
-                        }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= UNSCALE;
+                for (int j = 0; j < 4; ++j) v[j] *= UNSCALE;
                 const Terms t = terms_of(v);
-                const u32 to = a0 + (c >> 6) * 2 * SLICE + swizzled(r, (c & 63) >> 3);
+                const u32 to = a0 + (c >> 6) * 2 * SLICE + swizzled(r, (c & 63) >> 3) + 2 * (c & 4);
                 for (int i = 0; i < active; ++i) {
-                    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(in_block(to, i)), "r"(t.h.x), "r"(t.h.y), "r"(t.h.z), "r"(t.h.w) : "memory");
-                    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(in_block(to + SLICE, i)), "r"(t.l.x), "r"(t.l.y), "r"(t.l.z), "r"(t.l.w) : "memory");
+                    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(in_block(to, i)), "r"(t.h.x), "r"(t.h.y) : "memory");
+                    asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(in_block(to + SLICE, i)), "r"(t.l.x), "r"(t.l.y) : "memory");
                 }
             }
             cluster_barrier_async();
