@@ -39,7 +39,7 @@ __device__ __forceinline__ float max_nan(float x, float y) {
     return z;
 }
 // exp of d <= 0, by the fast form: its argument is rounded once, |d| U of the result, and in a sum the terms of large |d| are small.
-// (The exact form takes five instructions more, of about ten that a value takes in all; 2.4 M x 47: 317 us instead of ...)
+// (A tile kernel with the exact form: 2.4 M x 47 fp32 115 us, with this one 102.)
 __device__ __forceinline__ float exp_of(float d) { return __expf(d); }
 
 struct ForwardParams {
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(TILE_THREADS) tile_kernel(const ForwardParams 
 }
 
 // ---- long rows ------------------------------------------------------------------------------------
-constexpr int THREADS = 256, WARPS = THREADS / 32, CLUSTER = 8;
+constexpr int CLUSTER = 8;
 constexpr int LISTED = 512;  // candidates for the list that a block keeps
 
 // A part of a row: its largest value m and s = sum exp(x - m), t = sum exp(x - m) (m - x) over all of it.
@@ -292,7 +292,7 @@ union Vector {
 
 // Calls f(first, value) for single values and g(first, values) for batches of up to BATCH vectors, BATCH vectors N values, of [a, b)
 // of x that fall to this thread.
-template <class T>
+template <class T, int THREADS>
 struct Stretch {
     static constexpr int N = Vector<T>::N, BATCH = 4;
     const T* x;
@@ -352,8 +352,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 // For the list, the top-th largest of the largest values of 32 groups of threads bounds the last place from below: the values that
 // reach it, not many more than the list is long, are collected in a second pass (out of L2) and ranked by comparing each with all.
 // Where equal values make them too many, the list is found by one pass for each place.
-template <class T>
+// THREADS: 256, or 128 for rows of less than 32 KB, of which more are then under way (30 000 rows of 2 000 fp32, 3 best: 256 -> 209 us).
+template <class T, int THREADS>
 __global__ void __launch_bounds__(THREADS) long_kernel(const ForwardParams p) {
+    constexpr int WARPS = THREADS / 32, GROUP = THREADS / 32;  // (32 groups of so many threads)
     __shared__ __align__(16) float s_max[WARPS];
     __shared__ float2 s_sum[WARPS];
     __shared__ float s_group[32], s_others[WARPS];
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(THREADS) long_kernel(const ForwardParams p) {
     const int a = min(rank * each, p.c), b = min(a + each, p.c);
     const int64_t row = blockIdx.x / blocks;
     const T* x = static_cast<const T*>(p.x) + row * p.ld;
-    const Stretch<T> part(x, a, b);
+    const Stretch<T, THREADS> part(x, a, b);
 
     Part mine{-INFINITY, 0.f, 0.f, 0.f};
     part.run(
@@ -403,13 +405,13 @@ __global__ void __launch_bounds__(THREADS) long_kernel(const ForwardParams p) {
             mine.s += s.x + s.y;
             mine.t -= t.x + t.y;
         });
-    // the block's largest value; on the way there, those of groups of 8 threads
+    // the block's largest value; on the way there, those of groups of threads
     float m = mine.m;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, o));
-    if (lane % 8 == 0) s_group[warp * 4 + lane / 8] = m;
+    for (int o = 1; o < GROUP; o <<= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, o));
+    if (lane % GROUP == 0) s_group[(int)threadIdx.x / GROUP] = m;
 #pragma unroll
-    for (int o = 8; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, o));
+    for (int o = GROUP; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(FULL, m, o));
     if (lane == 0) s_max[warp] = m;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(THREADS) long_kernel(const ForwardParams p) {
             if (v < m) sum += exp_of(fmaxf(v - m, LOWEST));
             else equal += 1.f;
         };
-        const Stretch<T> whole(x, 0, p.c);
+        const Stretch<T, THREADS> whole(x, 0, p.c);
         whole.run(add, [&](const auto& w, auto batch, int) {
 #pragma unroll
             for (int k = 0; k < decltype(batch)::value; ++k)
@@ -667,43 +669,46 @@ __global__ void __launch_bounds__(256) rows_grad_kernel(const BackwardParams p) 
         }
 }
 
-// Long rows: a block to a stretch of STRETCH classes of a row.
-constexpr int STRETCH = 4096;
+// Long rows: a block to a stretch of a row, four vectors a thread, which are on their way before anything else is asked for.
+constexpr int THREADS = 256;
+constexpr int stretch_of(int size) { return 4 * THREADS * 16 / size; }
 
 template <class T>
 __global__ void __launch_bounds__(THREADS) long_grad_kernel(const BackwardParams p, const int stretches) {
-    constexpr int N = Vector<T>::N;
+    constexpr int N = Vector<T>::N, EACH = 4, STRETCH = EACH * THREADS * N;
     cbm::wait_before();
     const int64_t row = blockIdx.x / stretches;
     const int a = (int)(blockIdx.x % stretches) * STRETCH, b = min(a + STRETCH, p.c);
     const T* x = static_cast<const T*>(p.x) + row * p.ld;
     T* dx = static_cast<T*>(p.dx) + row * p.ld_out;
+    const bool alike = ((reinterpret_cast<u64>(x) ^ reinterpret_cast<u64>(dx)) & 15) == 0;
+    const int off = (int)(((16 - (reinterpret_cast<u64>(x + a) & 15)) & 15) / sizeof(T));
+    const int head = min(off, b - a), vectors = (b - a - head) / N, done = a + head + vectors * N;
+    Vector<T> w[EACH];
+    if (alike) {
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if ((int)threadIdx.x + k * THREADS < vectors) w[k].bits = reinterpret_cast<const uint4*>(x + a + head)[threadIdx.x + k * THREADS];
+    }
     const RowGradient<T> g(p, row);
     auto one = [&](int j) {
         const float d = g.base(cbm::widen(x[j]));
         dx[j] = cbm::narrow<T>(j == g.label ? d + g.gl : d);
     };
-    if (((reinterpret_cast<u64>(x) ^ reinterpret_cast<u64>(dx)) & 15) == 0) {
-        const int off = (int)(((16 - (reinterpret_cast<u64>(x + a) & 15)) & 15) / sizeof(T));
-        const int head = min(off, b - a), vectors = (b - a - head) / N, done = a + head + vectors * N;
+    if (alike) {
         if ((int)threadIdx.x < head) one(a + threadIdx.x);
-        constexpr int EACH = STRETCH / N / THREADS;
-        Vector<T> w[EACH];
-#pragma unroll
-        for (int k = 0; k < EACH; ++k)
-            if ((int)threadIdx.x + k * THREADS < vectors) w[k].bits = reinterpret_cast<const uint4*>(x + a + head)[threadIdx.x + k * THREADS];
+        if ((int)threadIdx.x < b - done) one(done + threadIdx.x);
 #pragma unroll
         for (int k = 0; k < EACH; ++k)
             if ((int)threadIdx.x + k * THREADS < vectors) {
-                const int j0 = a + head + (threadIdx.x + k * THREADS) * N;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float d = g.base(cbm::widen(w[k].v[i]));
-                    w[k].v[i] = cbm::narrow<T>(j0 + i == g.label ? d + g.gl : d);
-                }
+                for (int i = 0; i < N; ++i) w[k].v[i] = cbm::narrow<T>(g.base(cbm::widen(w[k].v[i])));
                 reinterpret_cast<uint4*>(dx + a + head)[threadIdx.x + k * THREADS] = w[k].bits;
             }
-        if ((int)threadIdx.x < b - done) one(done + threadIdx.x);
+        if (g.label >= a + head && g.label < done) {  // (one of the vectors': put right behind them)
+            __syncthreads();
+            if (threadIdx.x == 0) dx[g.label] = cbm::narrow<T>(g.base(cbm::widen(x[g.label])) + g.gl);
+        }
     } else {
         for (int j = a + threadIdx.x; j < b; j += THREADS) one(j);
     }
@@ -720,8 +725,8 @@ constexpr int ROW_MAX = 1024;  // classes that 32 lanes hold in registers, 32 ea
 int check(const char* who, int64_t n, int64_t ld, int32_t c, int32_t top, int32_t type) {
     if (n < 0 || c < 1 || ld < c || top < 0 || top > CBM_B200_MAX_TOP || top > c || type < 0 || type > CBM_B200_FP16)
         return cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes or type");
-    // (a grid has at most 2^31 - 1 blocks: a row to 32 lanes, or to a block for every STRETCH classes)
-    if (n > ((int64_t)1 << 31) - 1 || (c > ROW_MAX && n * ((c + STRETCH - 1) / STRETCH) > ((int64_t)1 << 31) - 1))
+    // (a grid has at most 2^31 - 1 blocks: a row to 32 lanes, or to a block for every stretch of 4 096 classes)
+    if (n > ((int64_t)1 << 31) - 1 || (c > ROW_MAX && n * ((c + 4095) / 4096) > ((int64_t)1 << 31) - 1))
         return cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": more rows than a launch has blocks for");
     return CBM_B200_OK;
 }
@@ -782,7 +787,7 @@ int blocks_to_row(int64_t n, int c, int32_t type) {
 }
 
 template <class P>
-void launch_clusters(void (*kernel)(P), int64_t blocks, int cluster, const cbm::Stream& on, const P& p) {
+void launch_clusters(void (*kernel)(P), int64_t blocks, int cluster, int threads, const cbm::Stream& on, const P& p) {
     cudaLaunchAttribute attrs[2] = {};
     attrs[0].id = cudaLaunchAttributeClusterDimension;
     attrs[0].val.clusterDim.x = cluster;
@@ -791,7 +796,7 @@ void launch_clusters(void (*kernel)(P), int64_t blocks, int cluster, const cbm::
     attrs[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)blocks);
-    config.blockDim = dim3(THREADS);
+    config.blockDim = dim3(threads);
     config.stream = on.s;
     config.attrs = attrs;
     config.numAttrs = on.captured ? 1 : 2;
@@ -822,7 +827,8 @@ extern "C" int cbm_b200_class_log_probs(const void* logits, int64_t ld, int32_t 
         }
         if (n_classes > ROW_MAX) {
             const int k = blocks_to_row(n_rows, n_classes, type);
-            launch_clusters(long_kernel<T>, n_rows * k, k, on, p);
+            if (k == 1 && n_classes * (int64_t)sizeof(T) < 32 * 1024) launch_clusters(long_kernel<T, 128>, n_rows, 1, 128, on, p);
+            else launch_clusters(long_kernel<T, 256>, n_rows * k, k, 256, on, p);
             return;
         }
         const int values = n_classes <= 256 ? 8 : 32;
@@ -858,7 +864,7 @@ extern "C" int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int
                 cbm::launch_next(kernel, dim3(blocks_of(n_rows, tile.rows)), TILE_THREADS, tile.bytes, on, p, tile);
             });
         } else if (n_classes > ROW_MAX) {
-            const int stretches = (n_classes + STRETCH - 1) / STRETCH;
+            const int stretch = stretch_of(sizeof(T)), stretches = (n_classes + stretch - 1) / stretch;
             cbm::launch_next(long_grad_kernel<T>, dim3((unsigned)(n_rows * stretches)), THREADS, 0, on, p, stretches);
         } else {
             p.shift = lanes_for(n_classes, 8);
