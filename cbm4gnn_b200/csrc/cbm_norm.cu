@@ -965,7 +965,10 @@ struct Plan {
         int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
         if (teams < 1) teams = 1;
         tile = (n_rows + teams - 1) / teams;
-        if (tile < 8 * at_once) tile = 8 * at_once;
+        // At least eight turns, or where samples are shorter than a turn as much as eight of them (198 071 x 4 bf16, samples of 4 rows, with
+        // the gradient: 491 -> 233 us).
+        const int64_t mean = n_samples ? n_rows / n_samples + 1 : n_rows + 1, least = 8 * (mean < at_once ? mean : at_once);
+        if (tile < least) tile = least;
         tiles = (n_rows + tile - 1) / tile;
         parts = tiles;
         joins = ptr || rows_each > tile;
