@@ -276,6 +276,7 @@ struct Team {
     int groups, vectors, at_once;      // of the slab; threads of its rows, rows at once
     int group0, row_in, group, lane;   // this thread's; row_in >= at_once: none
     int channel, there;                // first of its values, and how many
+    bool flat;                         // a warp whose groups' threads are told apart by bits of their numbers
     __device__ __forceinline__ Team(const Params& p, int E, bool strided) {
         size = p.team;
         id = threadIdx.x / size, thread = threadIdx.x % size;
@@ -289,6 +290,18 @@ struct Team {
         else lane = thread % vectors % p.lanes;
         channel = group * p.width + (strided ? lane : lane * E);
         there = strided ? (p.width - lane + p.lanes - 1) / p.lanes : E;
+        flat = size == 32 && !(p.lanes & (p.lanes - 1)) && !(vectors & (vectors - 1));
+    }
+    // Rows, of `rows`, of row r of those at work at once: one division for all of them.
+    __device__ __forceinline__ int turns(int rows, int r) const {
+        const u32 each = (u32)rows / (u32)at_once;
+        return (int)each + (r < rows - (int)each * at_once);
+    }
+    // Sum over a group's threads, flat teams only: all of them get it.
+    __device__ __forceinline__ float flat_sum(float v, int lanes) const {
+        for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(FULL, v, o);
+        for (int o = vectors; o < 32; o <<= 1) v += __shfl_xor_sync(FULL, v, o);
+        return v;
     }
     __device__ __forceinline__ bool on() const { return row_in < at_once; }
     __device__ __forceinline__ void sync() const {
@@ -305,15 +318,13 @@ struct Join {
     const Team& t;
     const float2* part;  // of the group
     int rows;
-    // Rows of thread r of those that are at work on a column.
-    __device__ __forceinline__ int rows_of(int r) const { return (rows - r + t.at_once - 1) / t.at_once; }
     // By one thread: f(what a thread left, how many values it is of).
     template <class F>
     __device__ __forceinline__ void alone(F&& f) const {
         const int most = min(t.at_once, rows);
         const float2* at = part;
         for (int r = 0; r < most; ++r, at += t.vectors) {
-            const int n = rows_of(r);
+            const int n = t.turns(rows, r);
             const float full = (float)(n * E);
             for (int l = 0; l < p.lanes; ++l) f(at[l], STRIDED ? (float)(n * values_of<E, STRIDED>(l, p.lanes, p.width)) : full);
         }
@@ -324,7 +335,7 @@ struct Join {
         const int entries = min(t.at_once, rows) * p.lanes;
         for (int i = threadIdx.x & 31; i < entries; i += 32) {
             const int r = i / p.lanes, l = i - r * p.lanes;
-            f(part[r * t.vectors + l], (float)(rows_of(r) * values_of<E, STRIDED>(l, p.lanes, p.width)));
+            f(part[r * t.vectors + l], (float)(t.turns(rows, r) * values_of<E, STRIDED>(l, p.lanes, p.width)));
         }
     }
     template <bool WARP>
@@ -349,6 +360,14 @@ struct Join {
         return s;
     }
 };
+// The same out of registers, by a flat team.
+template <bool MEANS>
+__device__ __forceinline__ float2 joined_flat(const Params& p, const Team& t, float2 mine, int rows) {
+    if constexpr (!MEANS) return float2{t.flat_sum(mine.x, p.lanes), t.flat_sum(mine.y, p.lanes)};
+    const float ref = __shfl_sync(FULL, mine.x, (t.group - t.group0) * p.lanes), n = (float)(t.turns(rows, t.row_in) * t.there);
+    const float mean = ref + t.flat_sum(n * (mine.x - ref), p.lanes) / ((float)rows * (float)p.width);
+    return float2{mean, t.flat_sum(mine.y + n * (mine.x - mean) * (mine.x - mean), p.lanes)};
+}
 // A group of few threads is joined by each of them for itself, which saves the way through shared memory and a barrier.
 constexpr int FEW = 32;
 
@@ -366,7 +385,7 @@ __host__ __device__ constexpr int batch_of() {
 // fetched without a question about each, the last one again in place of those that are not there: as branches the fetches would come
 // one after the other.
 template <class T, int E, bool STRIDED, bool GRAD, class F>
-__device__ __forceinline__ void for_rows(const T* x, const T* gy, int64_t dx, int64_t dg, int64_t count, int lanes, int there, F&& f) {
+__device__ __forceinline__ void for_rows(const T* x, const T* gy, int64_t dx, int64_t dg, int count, int lanes, int there, F&& f) {
     constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
     Values<T, E, STRIDED> v[BATCH], g[GRAD ? BATCH : 1];
     for (; count >= BATCH; count -= BATCH) {
@@ -378,7 +397,7 @@ __device__ __forceinline__ void for_rows(const T* x, const T* gy, int64_t dx, in
         f(v, g, All<BATCH>());
     }
     if (count > 0) {
-        const int have = (int)count;
+        const int have = count;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
             v[k].load(x, lanes, there);
@@ -413,8 +432,8 @@ __device__ __forceinline__ void write_rows(const Params& p, const Team& t, int64
                                            float2 stat, float2 sums) {
     const int64_t first = lo + t.row_in;
     if (!t.on() || first >= hi) return;
-    const int64_t count = (hi - first + t.at_once - 1) / t.at_once;
-    const int64_t begin = BACK ? first + (count - 1) * t.at_once : first, step = BACK ? -t.at_once : t.at_once;
+    const int count = t.turns((int)(hi - lo), t.row_in);  // (at most two tiles, or a block's part of a short sample: they fit 31 bits)
+    const int64_t begin = BACK ? first + (int64_t)(count - 1) * t.at_once : first, step = BACK ? -t.at_once : t.at_once;
     T* y = static_cast<T*>(p.y) + t.channel + begin * p.ldy;
     const int64_t dy = step * p.ldy;
     with_activation(p.act, [&](auto act) {
@@ -457,7 +476,7 @@ __device__ __forceinline__ float2 gathered(const Params& p, const Team& t, int64
     for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
     auto rows_of = [&](auto&& f) {
         for_rows<T, E, STRIDED, GRAD>(x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
-                                      (rows - t.row_in + t.at_once - 1) / t.at_once, p.lanes, t.there, f);
+                                      t.turns(rows, t.row_in), p.lanes, t.there, f);
     };
     if constexpr (GRAD) {
         with_activation(p.act, [&](auto act) {
@@ -572,8 +591,11 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
         const int rows = (int)(hi - lo);  // (at most two tiles, which fit 31 bits)
         float2 at{0.f, 0.f};
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-        part[t.thread] = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
-        t.sync();
+        const float2 mine = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
+        if (!t.flat) {
+            part[t.thread] = mine;
+            t.sync();
+        }
         const float share = 1.f / ((float)rows * (float)p.width);
         const bool whole = e - a <= p.tile;
         // for a group: what was found, from its threads' joined parts
@@ -592,7 +614,9 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
             return found;
         };
         float2 found{0.f, 0.f};
-        if (p.lanes * t.at_once <= FEW) {
+        if (t.flat) {
+            found = finish(t.group, joined_flat<!GRAD>(p, t, mine, rows), t.row_in == 0 && t.lane == 0);
+        } else if (p.lanes * t.at_once <= FEW) {
             const Join<!GRAD, E, STRIDED> join{p, t, part + (t.group - t.group0) * p.lanes, rows};
             found = finish(t.group, join.template run<false>(), t.row_in == 0 && t.lane == 0);
             part = part == s_part[0] + t.id * t.size ? s_part[1] + t.id * t.size : s_part[0] + t.id * t.size;
@@ -616,9 +640,10 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
     }
 }
 
-// The pieces of each sample that is longer than a tile, JOINERS threads to a group.  Block x: a tile, for the sample that starts in it, or
-// where samples are equal, a sample; y: the groups y, y + gridDim.y, ...  The blocks behind add up the channels' sums, 32 each.
-constexpr int JOINERS = 256;
+// The pieces of each sample that is longer than a tile: by a warp, or where they are many by a block.  Block x: JOINED tiles, for the samples
+// that start in them, or where samples are equal, JOINED samples; y: the groups y, y + gridDim.y, ...  The blocks behind add up the channels'
+// sums, CHANNELS each.
+constexpr int JOINERS = 256, JOINED = JOINERS / 32, MANY = 128, CHANNELS = 4;
 
 __device__ __forceinline__ float joiners_sum(float v, float* s_sum) {
     v = lanes_sum(v, 32);
@@ -631,72 +656,92 @@ __device__ __forceinline__ float joiners_sum(float v, float* s_sum) {
     return v;
 }
 
+// Sample s, which starts in `tile`, [a, e), by the threads `at` of `size`, whose values `sum` adds up.
+template <bool GRAD, class Sum>
+__device__ __forceinline__ void join_sample(const Params& p, int64_t s, int64_t a, int64_t e, int at, int size, Sum&& sum) {
+    const int64_t tile = a / p.tile, last = (e - 1) / p.tile;
+    const float count = (float)(e - a) * (float)p.width;
+    for (int g = blockIdx.y; g < p.groups; g += gridDim.y) {
+        const float2* found = p.pieces + (int64_t)g * p.tiles;
+        // of the first tile it is the second piece unless the sample starts with the tile
+        auto piece = [&](int64_t q) { return found[(q == tile && a > tile * p.tile ? p.groups * p.tiles : 0) + q]; };
+        if constexpr (GRAD) {
+            float2 all{0.f, 0.f};
+#pragma unroll 4
+            for (int64_t q = tile + at; q <= last; q += size) {
+                const float2 one = piece(q);
+                all.x += one.x, all.y += one.y;
+            }
+            all = float2{sum(all.x), sum(all.y)};
+            if (at == 0) p.joined[tile * p.groups + g] = float2{all.x / count, all.y / count};
+        } else {
+            auto rows = [&](int64_t q) { return (float)(min(e, (q + 1) * p.tile) - max(a, q * p.tile)); };
+            const float ref = piece(tile).x;
+            float m = 0.f, squares = 0.f;
+#pragma unroll 4
+            for (int64_t q = tile + at; q <= last; q += size) m += rows(q) * (piece(q).x - ref);
+            const float mean = ref + sum(m) / (float)(e - a);
+#pragma unroll 4
+            for (int64_t q = tile + at; q <= last; q += size) {
+                const float2 one = piece(q);
+                squares += one.y + rows(q) * (float)p.width * (one.x - mean) * (one.x - mean);
+            }
+            const float r = rsqrtf(sum(squares) / count + p.eps);
+            if (at == 0) {
+                p.joined[tile * p.groups + g] = float2{mean, r};
+                if (p.mean) {
+                    p.mean[s * p.groups + g] = mean;
+                    p.r[s * p.groups + g] = r;
+                }
+            }
+        }
+    }
+}
+
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(JOINERS) join_kernel(const Params p, const int64_t starts) {
     __shared__ float s_sum[JOINERS / 32];
+    __shared__ int64_t s_long[JOINED];
     cbm::wait_before();
-    if (blockIdx.x < starts) {
-        int64_t s = blockIdx.x, tile = blockIdx.x;
-        if (p.ptr) {
+    const int64_t blocks = (starts + JOINED - 1) / JOINED;
+    const int warp = threadIdx.x >> 5;
+    if (blockIdx.x < blocks) {
+        const int64_t mine = (int64_t)blockIdx.x * JOINED + warp;
+        int64_t s = mine < starts ? mine : -1, a = 0, e = 0;
+        if (p.ptr && s >= 0) {
             // (a sample that starts with the tile fills it)
-            s = p.longer[p.tiles + tile];
-            if (s < 0) s = p.longer[tile];
-            if (s < 0 || start_of(p, s) < tile * p.tile) return;
+            s = p.longer[p.tiles + mine];
+            if (s < 0) s = p.longer[mine];
         }
-        const int64_t a = start_of(p, s), e = start_of(p, s + 1);
-        tile = a / p.tile;
-        const int64_t last = (e - 1) / p.tile;
-        const float count = (float)(e - a) * (float)p.width;
-        for (int g = blockIdx.y; g < p.groups; g += gridDim.y) {
-            const float2* found = p.pieces + (int64_t)g * p.tiles;
-            // of the first tile it is the second piece unless the sample starts with the tile
-            auto piece = [&](int64_t q) { return found[(q == tile && a > tile * p.tile ? p.groups * p.tiles : 0) + q]; };
-            if constexpr (GRAD) {
-                float2 all{0.f, 0.f};
-#pragma unroll 4
-                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) {
-                    const float2 one = piece(q);
-                    all.x += one.x, all.y += one.y;
-                }
-                all = float2{joiners_sum(all.x, s_sum), joiners_sum(all.y, s_sum)};
-                if (threadIdx.x == 0) p.joined[tile * p.groups + g] = float2{all.x / count, all.y / count};
-            } else {
-                auto rows = [&](int64_t q) { return (float)(min(e, (q + 1) * p.tile) - max(a, q * p.tile)); };
-                const float ref = piece(tile).x;
-                float m = 0.f, squares = 0.f;
-#pragma unroll 4
-                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) m += rows(q) * (piece(q).x - ref);
-                const float mean = ref + joiners_sum(m, s_sum) / (float)(e - a);
-#pragma unroll 4
-                for (int64_t q = tile + threadIdx.x; q <= last; q += JOINERS) {
-                    const float2 one = piece(q);
-                    squares += one.y + rows(q) * (float)p.width * (one.x - mean) * (one.x - mean);
-                }
-                const float r = rsqrtf(joiners_sum(squares, s_sum) / count + p.eps);
-                if (threadIdx.x == 0) {
-                    p.joined[tile * p.groups + g] = float2{mean, r};
-                    if (p.mean) {
-                        p.mean[s * p.groups + g] = mean;
-                        p.r[s * p.groups + g] = r;
-                    }
-                }
-            }
+        if (s >= 0) {
+            a = start_of(p, s), e = start_of(p, s + 1);
+            if (p.ptr && a < mine * p.tile) s = -1;
+        }
+        const bool many = s >= 0 && e - a > MANY * p.tile;
+        if (s >= 0 && !many) join_sample<GRAD>(p, s, a, e, threadIdx.x & 31, 32, [](float v) { return lanes_sum(v, 32); });
+        if ((threadIdx.x & 31) == 0) s_long[warp] = many ? s : -1;
+        if (!__syncthreads_or(many)) return;
+        for (int i = 0; i < JOINED; ++i) {
+            s = s_long[i];
+            if (s >= 0) join_sample<GRAD>(p, s, start_of(p, s), start_of(p, s + 1), threadIdx.x, JOINERS, [&](float v) { return joiners_sum(v, s_sum); });
         }
     } else if constexpr (GRAD) {
         if (blockIdx.y) return;
-        __shared__ float2 s_part[JOINERS / 32][33];
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (int)(blockIdx.x - starts) * 32 + lane;
+        __shared__ float2 s_part[JOINED][CHANNELS];
+        const int column = threadIdx.x % CHANNELS, c = (int)(blockIdx.x - blocks) * CHANNELS + column;
         float2 all{0.f, 0.f};
         if (c < p.c)
 #pragma unroll 8
-            for (int64_t q = warp; q < p.parts; q += JOINERS / 32) {
+            for (int64_t q = threadIdx.x / CHANNELS; q < p.parts; q += JOINERS / CHANNELS) {
                 const float2 one = p.channels[q * p.c + c];
                 all.x += one.x, all.y += one.y;
             }
-        s_part[warp][lane] = all;
+#pragma unroll
+        for (int o = CHANNELS; o < 32; o <<= 1) all.x += __shfl_xor_sync(FULL, all.x, o), all.y += __shfl_xor_sync(FULL, all.y, o);
+        if ((threadIdx.x & 31) < CHANNELS) s_part[warp][column] = all;
         __syncthreads();
-        if (warp == 0 && c < p.c) {
-            for (int i = 1; i < JOINERS / 32; ++i) all.x += s_part[i][lane].x, all.y += s_part[i][lane].y;
+        if (threadIdx.x < CHANNELS && c < p.c) {
+            for (int i = 1; i < JOINED; ++i) all.x += s_part[i][column].x, all.y += s_part[i][column].y;
             if (p.gw) p.gw[c] = all.x;
             if (p.gb) p.gb[c] = all.y;
         }
@@ -965,9 +1010,8 @@ struct Plan {
         int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
         if (teams < 1) teams = 1;
         tile = (n_rows + teams - 1) / teams;
-        // At least eight turns, or where samples are shorter than a turn as much as eight of them (198 071 x 4 bf16, samples of 4 rows, with
-        // the gradient: 491 -> 233 us).
-        const int64_t mean = n_samples ? n_rows / n_samples + 1 : n_rows + 1, least = 8 * (mean < at_once ? mean : at_once);
+        // At least two turns, or where samples are shorter than a turn as much as two of them.
+        const int64_t mean = n_samples ? n_rows / n_samples + 1 : n_rows + 1, least = 2 * (mean < at_once ? mean : at_once);
         if (tile < least) tile = least;
         tiles = (n_rows + tile - 1) / tile;
         parts = tiles;
@@ -1052,7 +1096,7 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
             if (!plan.joins) return;
             joins = p.ptr ? p.tiles : p.n_samples;
             const int across = p.ptr ? (p.groups < 4 ? p.groups : 4) : p.groups;  // (most blocks of tiles find nothing to do)
-            cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)(joins + (sums ? (p.c + 31) / 32 : 0)), across), JOINERS, 0, on, p, joins);
+            cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)((joins + JOINED - 1) / JOINED + (sums ? (p.c + CHANNELS - 1) / CHANNELS : 0)), across), JOINERS, 0, on, p, joins);
             cbm::launch_next(long_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
         });
     } else {
@@ -1061,7 +1105,7 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
         if (p.ptr) cbm::launch_next(outside_kernel<T>, blocks_for(p.n_rows), THREADS, 0, on, p);
         if (sums) cbm::launch_next(wide_params_kernel<T>, dim3((unsigned)p.parts, (p.c + THREADS - 1) / THREADS), THREADS, 0, on, p);
     }
-    if (sums && !joins) cbm::launch_next(join_kernel<T, true>, dim3((p.c + 31) / 32), JOINERS, 0, on, p, joins);
+    if (sums && !joins) cbm::launch_next(join_kernel<T, true>, dim3((p.c + CHANNELS - 1) / CHANNELS), JOINERS, 0, on, p, joins);
 }
 
 // Workspace of a call, whatever the type and the alignment of its rows.
