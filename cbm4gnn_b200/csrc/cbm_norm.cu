@@ -379,7 +379,7 @@ struct All {
 // Rows that a thread fetches at a time.
 template <class T, int E, bool STRIDED, bool GRAD>
 __host__ __device__ constexpr int batch_of() {
-    return STRIDED ? (E == 1 ? 8 : E == 4 || !GRAD ? 4 : 2) : E * sizeof(T) >= 8 ? 4 : 8;
+    return STRIDED ? (E == 1 ? 8 : E == 4 || !GRAD ? 4 : 2) : E == 8 && GRAD ? 2 : E * sizeof(T) >= 8 ? 4 : 8;
 }
 // Calls f(values, values of the gradient, how many rows) for the `count` rows from x on, `dx` apart, a batch at a time.  The last rows are
 // fetched without a question about each, the last one again in place of those that are not there: as branches the fetches would come
