@@ -4,13 +4,15 @@
 // a sample's group:  xh = (x - mean) r,  z = w xh + b,  y = act(z).
 // Gradients, with g = gy act'(z) and u = w g:  gb = sum g,  gw = sum g xh,  gx = r (u - mean(u) - xh mean(u xh)).
 //
-// What bounds all of it is memory: x is read and y written once, x and gy are read and gx written once.  Three ways:
+// What bounds all of it is memory: x is read and y written once, x and gy are read and gx written once.  The ways:
 //   * Samples of one row: lanes hold their part of a group in registers; nothing is read twice, and the gradient computes the
 //     statistics anew instead of reading them.
-//   * Samples of up to a tile's rows: a team of threads reads a sample, joins its sums in shared memory and reads it again, out of L1 or
-//     L2, to write the results.  Tiles end where samples do, so that each of these is one team's.
-//   * Longer samples: every tile leaves a partial result, one warp to a group joins them in a fixed order, and a third kernel
+//   * Samples of up to a tile's rows: a team of threads reads a sample, joins its sums in registers or shared memory and reads it again,
+//     out of L1 or L2, to write the results.  Tiles end where samples do, so that each of these is one team's.
+//   * Longer samples: every tile leaves a partial result, a warp or a block to a sample joins them in a fixed order, and a third kernel
 //     goes over the rows again, from their ends, which L2 still holds.
+//   * A few samples of some hundred rows: a cluster of blocks to each, which join through one another's shared memory: one launch.
+//   * Groups wider than a block's threads hold: a block to each, value by value.
 // Means and squares around them are kept for every few rows and joined (mean and sum of squares around it of two parts give those of
 // both), so that a mean far from 0 costs no digits; no sum depends on the order in which blocks run.
 #include "cbm_common.h"
@@ -376,35 +378,84 @@ template <int N>
 struct All {
     __device__ __forceinline__ constexpr operator int() const { return N; }
 };
-// Rows that a thread fetches at a time.
+// The gradient's vectors of 16 bytes come through shared memory, where each thread has DEPTH places of its own: rows ahead take no registers,
+// the code of a turn is that of one row, and the rows of a short sample are still there when they are asked for again.  (1 000 000 x 64 bf16 in
+// samples of 2 300 rows, with the gradient 465 -> 364 us; 235 868 x 256 fp32 350 -> 346.  Narrower vectors lose: 262 147 x 100 bf16 by pairs
+// 262 -> 290; so does the forward pass, whose turns are short: 102 -> 143.)
+template <class T, int E, bool STRIDED, bool GRAD>
+struct Ring {
+    static constexpr int VECTOR = E * sizeof(T), DEPTH = 4;
+    static constexpr bool ON = GRAD && !STRIDED && VECTOR == 16;
+    static constexpr int ROWS = ON ? DEPTH * 2 * VECTOR : 0, CHANNELS = GRAD ? 8 * E : 0;
+    static constexpr int EACH = ROWS > CHANNELS ? ROWS : CHANNELS;  // bytes to a thread; behind its rows, a team's channels' sums use them
+    static constexpr int BYTES = EACH ? EACH * THREADS : 16;
+    unsigned char *team, *at;  // this team's places, this thread's first
+    int apart;
+    __device__ __forceinline__ Ring(unsigned char* smem, const Team& t)
+        : team(smem + t.id * t.size * EACH), at(team + t.thread * VECTOR), apart(t.size * VECTOR) {}
+    __device__ __forceinline__ unsigned char* place(int row, int which) const { return at + ((row & (DEPTH - 1)) * 2 + which) * apart; }
+    __device__ __forceinline__ void copy(const T* from, int row, int which) const {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((u32)__cvta_generic_to_shared(place(row, which))), "l"(from), "n"(VECTOR) : "memory");
+    }
+    // Whether `count` rows that were gone over are all there.
+    __device__ __forceinline__ bool keeps(int count) const { return ON && count <= DEPTH; }
+};
+// Rows that a thread takes at a time: out of its places one, else as many as it fetches.
 template <class T, int E, bool STRIDED, bool GRAD>
 __host__ __device__ constexpr int batch_of() {
-    return STRIDED ? (E == 1 ? 8 : E == 4 || !GRAD ? 4 : 2) : E == 8 && GRAD ? 2 : E * sizeof(T) >= 8 ? 4 : 8;
+    return Ring<T, E, STRIDED, GRAD>::ON ? 1 : STRIDED ? (E == 1 ? 8 : E == 4 || !GRAD ? 4 : 2) : E * sizeof(T) >= 8 ? 4 : 8;
 }
-// Calls f(values, values of the gradient, how many rows) for the `count` rows from x on, `dx` apart, a batch at a time.  The last rows are
-// fetched without a question about each, the last one again in place of those that are not there: as branches the fetches would come
-// one after the other.
+// Calls f(values, values of the gradient, how many rows) for the `count` rows from x on, `dx` apart, a batch at a time; where `kept`, they are
+// in their places already.  The last rows of a fetch are fetched without a question about each, the last one again in place of those that are
+// not there: as branches the fetches would come one after the other.
 template <class T, int E, bool STRIDED, bool GRAD, class F>
-__device__ __forceinline__ void for_rows(const T* x, const T* gy, int64_t dx, int64_t dg, int count, int lanes, int there, F&& f) {
+__device__ __forceinline__ void for_rows(const Ring<T, E, STRIDED, GRAD>& ring, bool kept, const T* x, const T* gy, int64_t dx, int64_t dg, int count,
+                                         int lanes, int there, F&& f) {
     constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
     Values<T, E, STRIDED> v[BATCH], g[GRAD ? BATCH : 1];
-    for (; count >= BATCH; count -= BATCH) {
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-            v[k].load(x, lanes, there), x += dx;
-            if constexpr (GRAD) g[k].load(gy, lanes, there), gy += dg;
+    if constexpr (Ring<T, E, STRIDED, GRAD>::ON) {
+        constexpr int AHEAD = Ring<T, E, STRIDED, GRAD>::DEPTH - 1;
+        int asked = 0;
+        auto ask = [&] {  // (a group of copies for each row, where there are no more an empty one)
+            if (asked < count) {
+                ring.copy(x, asked, 0), x += dx;
+                ring.copy(gy, asked, 1), gy += dg;
+            }
+            ++asked;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        if (!kept)
+#pragma unroll 1
+            while (asked < AHEAD) ask();
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            if (!kept) {
+                ask();  // into the place of the row before this one, which is done with
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory");
+            }
+            v[0].bits = *reinterpret_cast<const uint4*>(ring.place(i, 0));
+            g[0].bits = *reinterpret_cast<const uint4*>(ring.place(i, 1));
+            f(v, g, All<1>());
         }
-        f(v, g, All<BATCH>());
-    }
-    if (count > 0) {
-        const int have = count;
+    } else {
+        for (; count >= BATCH; count -= BATCH) {
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-            v[k].load(x, lanes, there);
-            if constexpr (GRAD) g[k].load(gy, lanes, there);
-            if (k + 1 < have) x += dx, gy += dg;
+            for (int k = 0; k < BATCH; ++k) {
+                v[k].load(x, lanes, there), x += dx;
+                if constexpr (GRAD) g[k].load(gy, lanes, there), gy += dg;
+            }
+            f(v, g, All<BATCH>());
         }
-        f(v, g, have);
+        if (count > 0) {
+            const int have = count;
+#pragma unroll
+            for (int k = 0; k < BATCH; ++k) {
+                v[k].load(x, lanes, there);
+                if constexpr (GRAD) g[k].load(gy, lanes, there);
+                if (k + 1 < have) x += dx, gy += dg;
+            }
+            f(v, g, have);
+        }
     }
 }
 
@@ -428,7 +479,7 @@ __device__ __forceinline__ Values<T, E, STRIDED> finished(const Values<T, E, STR
 
 // Rows [lo, hi) of a sample, from the last row to the first where BACK.
 template <class T, int E, bool STRIDED, bool GRAD, bool BACK>
-__device__ __forceinline__ void write_rows(const Params& p, const Team& t, int64_t lo, int64_t hi, const float (&w)[E], const float (&b)[E],
+__device__ __forceinline__ void write_rows(const Params& p, const Team& t, const Ring<T, E, STRIDED, GRAD>& ring, bool kept, int64_t lo, int64_t hi, const float (&w)[E], const float (&b)[E],
                                            float2 stat, float2 sums) {
     const int64_t first = lo + t.row_in;
     if (!t.on() || first >= hi) return;
@@ -437,10 +488,11 @@ __device__ __forceinline__ void write_rows(const Params& p, const Team& t, int64
     T* y = static_cast<T*>(p.y) + t.channel + begin * p.ldy;
     const int64_t dy = step * p.ldy;
     with_activation(p.act, [&](auto act) {
-        for_rows<T, E, STRIDED, GRAD>(static_cast<const T*>(p.x) + t.channel + begin * p.ldx, static_cast<const T*>(p.gy) + t.channel + begin * p.ldgy,
+        constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
+        for_rows<T, E, STRIDED, GRAD>(ring, kept && ring.keeps(count), static_cast<const T*>(p.x) + t.channel + begin * p.ldx, static_cast<const T*>(p.gy) + t.channel + begin * p.ldgy,
                                       step * p.ldx, step * p.ldgy, count, p.lanes, t.there, [&](const auto& v, const auto& g, auto have) {
 #pragma unroll
-            for (int k = 0; k < batch_of<T, E, STRIDED, GRAD>(); ++k) {
+            for (int k = 0; k < BATCH; ++k) {
                 const auto out = finished<T, E, STRIDED, GRAD, decltype(act)::value>(v[k], g[GRAD ? k : 0], w, b, stat, sums);
                 if (k < have) out.store(y, p.lanes, t.there), y += dy;
             }
@@ -458,13 +510,13 @@ __device__ __forceinline__ void fetch_params(const Params& p, const Team& t, flo
     }
 }
 
-// Blocks of an SM: what their registers leave room for without spilling.
+// Blocks of an SM: with one more their registers spill to a few hundred bytes a thread, with one fewer too little is on its way.
 constexpr int blocks_resident(int e, bool grad) { return e == 8 ? (grad ? 2 : 3) : e == 4 && grad ? 3 : 4; }
 
 // What a thread finds in `rows` rows of a sample from row lo on: the mean over its values and the squares around it; or, for the gradient,
 // its sums of u and u xh, and by channel those of g xh and g, added to gw and gb.
 template <class T, int E, bool STRIDED, bool GRAD>
-__device__ __forceinline__ float2 gathered(const Params& p, const Team& t, int64_t lo, int rows, const float (&w)[E], const float (&b)[E], float2 at,
+__device__ __forceinline__ float2 gathered(const Params& p, const Team& t, const Ring<T, E, STRIDED, GRAD>& ring, int64_t lo, int rows, const float (&w)[E], const float (&b)[E], float2 at,
                                            float (&gw)[E], float (&gb)[E]) {
     constexpr int BATCH = batch_of<T, E, STRIDED, GRAD>();
     const T *x = static_cast<const T*>(p.x) + t.channel, *gy = static_cast<const T*>(p.gy) + t.channel;
@@ -475,7 +527,7 @@ __device__ __forceinline__ float2 gathered(const Params& p, const Team& t, int64
 #pragma unroll
     for (int i = 0; i < E; ++i) mean[i] = m2[i] = 0.f;
     auto rows_of = [&](auto&& f) {
-        for_rows<T, E, STRIDED, GRAD>(x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
+        for_rows<T, E, STRIDED, GRAD>(ring, false, x + (lo + t.row_in) * p.ldx, gy + (lo + t.row_in) * p.ldgy, t.at_once * p.ldx, t.at_once * p.ldgy,
                                       t.turns(rows, t.row_in), p.lanes, t.there, f);
     };
     if constexpr (GRAD) {
@@ -536,6 +588,7 @@ __device__ __forceinline__ float2 gathered(const Params& p, const Team& t, int64
 // A team's sums of g xh and g, as part `to`.
 template <class T, int E, bool STRIDED>
 __device__ __forceinline__ void store_channels(const Params& p, const Team& t, const float (&gw)[E], const float (&gb)[E], float2* s_channel, int64_t to) {
+    t.sync();  // (where the rows' places were)
 #pragma unroll
     for (int i = 0; i < E; ++i) s_channel[i * t.size + t.thread] = float2{gw[i], gb[i]};
     t.sync();
@@ -556,9 +609,10 @@ __device__ __forceinline__ void store_channels(const Params& p, const Team& t, c
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kernel(const Params p) {
     __shared__ float2 s_part[2][THREADS], s_stat[THREADS];  // (parts: of this sample and of the one before, which may still be read)
-    __shared__ float2 s_channel[GRAD ? THREADS * E : 1];
+    __shared__ __align__(16) unsigned char s_rows[Ring<T, E, STRIDED, GRAD>::BYTES];
     cbm::wait_before();
     const Team t(p, E, STRIDED);
+    const Ring<T, E, STRIDED, GRAD> ring(s_rows, t);
     const int64_t tile = (int64_t)blockIdx.x * (THREADS / p.team) + t.id;
     if (tile >= p.tiles) return;
     float2 *part = s_part[0] + t.id * t.size, *stat = s_stat + t.id * t.size;
@@ -591,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
         const int rows = (int)(hi - lo);  // (at most two tiles, which fit 31 bits)
         float2 at{0.f, 0.f};
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-        const float2 mine = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
+        const float2 mine = gathered<T, E, STRIDED, GRAD>(p, t, ring, lo, rows, w, b, at, gw, gb);
         if (!t.flat) {
             part[t.thread] = mine;
             t.sync();
@@ -633,10 +687,10 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) tiles_kerne
             if (t.thread == 0 && blockIdx.y == 0) p.longer[(a > tile * p.tile ? p.tiles : 0) + tile] = s;
             continue;
         }
-        write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, hi, w, b, GRAD ? at : found, found);
+        write_rows<T, E, STRIDED, GRAD, false>(p, t, ring, true, lo, hi, w, b, GRAD ? at : found, found);
     }
     if constexpr (GRAD) {
-        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, s_channel + t.id * t.size * E, tile);
+        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, reinterpret_cast<float2*>(ring.team), tile);
     }
 }
 
@@ -751,8 +805,10 @@ __global__ void __launch_bounds__(JOINERS) join_kernel(const Params p, const int
 // The rows of samples that are longer than a tile: at most two of them meet in one.
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) long_kernel(const Params p) {
+    __shared__ __align__(16) unsigned char s_rows[Ring<T, E, STRIDED, GRAD>::BYTES];
     cbm::wait_before();
     const Team t(p, E, STRIDED);
+    const Ring<T, E, STRIDED, GRAD> ring(s_rows, t);
     const int64_t tile = (int64_t)blockIdx.x * (THREADS / p.team) + t.id;
     if (tile >= p.tiles) return;
     float w[E], b[E];
@@ -766,24 +822,25 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) long_kernel
         const float2 found = p.joined[(a / p.tile) * p.groups + t.group];
         float2 at = found;
         if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-        if (lo < hi) write_rows<T, E, STRIDED, GRAD, true>(p, t, lo, hi, w, b, at, found);
+        if (lo < hi) write_rows<T, E, STRIDED, GRAD, true>(p, t, ring, false, lo, hi, w, b, at, found);
     }
 }
 
 // ---- a few samples that are not long: a cluster of blocks to each ----------------------------------
-constexpr int CLUSTER = 8;
+constexpr int CLUSTER = 8, GROUPS = 128;  // blocks to a sample; groups of a slab at most
 
 // Every block has a stretch of the sample's rows; what it finds goes to all blocks of the cluster, which read their rows again, out of L1 or
 // L2: one launch, where tiles, joins and rows take three.  y: a slab of groups.
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) cluster_kernel(const Params p) {
-    __shared__ float2 s_part[THREADS], s_stat[THREADS], s_all[CLUSTER][THREADS];
-    __shared__ float2 s_channel[GRAD ? THREADS * E : 1];
+    __shared__ float2 s_part[THREADS], s_stat[THREADS], s_all[CLUSTER][GROUPS];
+    __shared__ __align__(16) unsigned char s_rows[Ring<T, E, STRIDED, GRAD>::BYTES];
     u32 rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // the others' shared memory is there once all have started
     cbm::wait_before();
     const Team t(p, E, STRIDED);
+    const Ring<T, E, STRIDED, GRAD> ring(s_rows, t);
     const int64_t s = blockIdx.x / CLUSTER, each = (p.rows_each + CLUSTER - 1) / CLUSTER;
     auto rows_of = [&](int64_t k) { return (int)max(min(p.rows_each - k * each, each), (int64_t)0); };
     const int64_t lo = s * p.rows_each + min(rank * each, p.rows_each);
@@ -794,7 +851,7 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) cluster_ker
     for (int i = 0; i < E; ++i) gw[i] = gb[i] = 0.f;
     float2 at{0.f, 0.f};
     if constexpr (GRAD) at = float2{p.mean[s * p.groups + t.group], p.r[s * p.groups + t.group]};
-    s_part[t.thread] = gathered<T, E, STRIDED, GRAD>(p, t, lo, rows, w, b, at, gw, gb);
+    s_part[t.thread] = gathered<T, E, STRIDED, GRAD>(p, t, ring, lo, rows, w, b, at, gw, gb);
     __syncthreads();
     for (int g = t.thread >> 5; g < t.groups; g += THREADS / 32) {
         const Join<!GRAD, E, STRIDED> join{p, t, s_part + g * p.lanes, rows};
@@ -832,9 +889,9 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) cluster_ker
             p.r[s * p.groups + t.group] = found.y;
         }
     }
-    write_rows<T, E, STRIDED, GRAD, false>(p, t, lo, lo + rows, w, b, GRAD ? at : found, found);
+    write_rows<T, E, STRIDED, GRAD, false>(p, t, ring, true, lo, lo + rows, w, b, GRAD ? at : found, found);
     if constexpr (GRAD) {
-        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, s_channel, blockIdx.x);
+        if (p.channels) store_channels<T, E, STRIDED>(p, t, gw, gb, reinterpret_cast<float2*>(ring.team), blockIdx.x);
     }
 }
 
@@ -994,8 +1051,9 @@ struct Plan {
             return;
         }
         way = TILES;
-        slab_groups = THREADS / lanes < groups ? THREADS / lanes : groups;
-        // A few samples whose rows a cluster goes over in some dozen turns: 1 000 x 64 9 us, 15 with tiles, joins and rows by themselves.
+        slab_groups = THREADS / lanes < GROUPS ? THREADS / lanes : GROUPS;
+        if (groups < slab_groups) slab_groups = groups;
+        // A few samples whose rows a cluster goes over in some dozen turns: 1 000 x 64 fp32 12 us, 15 with tiles, joins and rows by themselves.
         const int64_t slabs = (groups + slab_groups - 1) / slab_groups, turn = (int64_t)CLUSTER * (THREADS / (slab_groups * lanes));
         if (!ptr && rows_each > 1 && n_samples * CLUSTER * slabs <= 2 * SMS && rows_each <= 48 * turn) {
             way = CLUSTERS;
@@ -1003,14 +1061,15 @@ struct Plan {
             parts = n_samples * CLUSTER;
             return;
         }
-        // Four rows at once, or where samples are short one, so that more of them are under way.
+        // Four rows at once, or where samples are short one, so that more of them are under way (262 147 x 100 bf16 in samples of 30 rows).
         const int wanted = (n_samples && n_rows / n_samples > 64 ? 4 : 1) * slab_groups * lanes;
         for (team = 32; team < THREADS && team < wanted;) team *= 2;
         const int at_once = team / (slab_groups * lanes);
         int64_t teams = (int64_t)SMS * blocks_resident(form.e, grad) * (THREADS / team) / slabs;  // resident at the same time
         if (teams < 1) teams = 1;
         tile = (n_rows + teams - 1) / teams;
-        // At least two turns, or where samples are shorter than a turn as much as two of them.
+        // At least two turns, or where samples are shorter than a turn as much as two of them (54 718 x 5 fp32, samples of 9 rows, with the
+        // gradient: eight turns 209 us, eight samples 158, two 111; 4 000 x 32 in samples of 23: 61 -> 52).
         const int64_t mean = n_samples ? n_rows / n_samples + 1 : n_rows + 1, least = 2 * (mean < at_once ? mean : at_once);
         if (tile < least) tile = least;
         tiles = (n_rows + tile - 1) / tile;
