@@ -87,6 +87,9 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
                 raise RuntimeError("orthogonal step: dense fp32 tensors expected")
             if t.device != dev:
                 raise RuntimeError(f"orthogonal step: operands on {dev} and {t.device}")
+    written = [t.data_ptr() for t in weights + momenta if t.numel() and t.device.type != "meta"]
+    if len(set(written)) < len(written):
+        raise RuntimeError("orthogonal step: a weight or a momentum is there twice")
     with torch.no_grad():
         if dev.type != "cuda":
             for w, g, m in zip(weights, grads, momenta):
