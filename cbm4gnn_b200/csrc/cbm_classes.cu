@@ -3,6 +3,9 @@
 // With m the largest of a row, s the sum of exp(x - m) over the others and t = sum exp(x - m) (m - x):
 //   log p_j = (x_j - m) - log1p(s),   entropy = log1p(s) + t / (1 + s).
 // Nothing in these is subtracted that is nearly equal, so a decided row keeps the digits of a log probability near 0.
+// What bounds it is memory: logits are read once, forwards and backwards, and the gradient is written once.  Narrow rows go through shared
+// memory, where lanes of a row lie a bank apart; long ones are gone over once by a block or a cluster, which keeps m, s and t as it goes
+// (2 449 029 x 47 fp32 102 us, 4.5 TB/s, with the gradient 244 us, of 152 at the rate of a copy).
 // Gradient: dx_j = g_log ([j = label] - p_j) - g_ent p_j (log p_j + entropy) + sum_i g_top_i ([j = c_i] - p_j).
 #include "cbm_common.h"
 #include "cbm_launch.cuh"
@@ -745,7 +748,9 @@ int lanes_for(int c, int values) {
     return shift;
 }
 
-constexpr int TILE_ROW = 4096;  // bytes of a row that goes through shared memory
+// Bytes of a row that goes through shared memory.  (With the gradient, fp32: 300 000 x 172 115 us, in registers 315; 100 000 x 1 000 221 us,
+// by a block each 420.)
+constexpr int TILE_ROW = 4096;
 
 // Values of a vector and the tile's layout for rows of `c` values at a pitch of `ld`; 0 where rows do not go that way.
 int tile_for(const void* x, int64_t ld, int c, int size, int* shift, Tile* t) {
@@ -779,7 +784,8 @@ void with_vector(int e, F&& f) {
     }
 }
 
-// Blocks to a row: while the rows alone leave SMs without one (two of them to each), and a part keeps 8 vectors a thread.
+// Blocks to a row: while the rows alone leave SMs without one (two of them to each), and a part keeps 8 vectors a thread.  (One row of
+// 128 256 fp32: 8 blocks 20.5 us, one 33; 32 rows of 30 000: 16.4, one 20.5.)
 int blocks_to_row(int64_t n, int c, int32_t type) {
     int k = 1;
     while (k < CLUSTER && n * k * 2 <= 2 * 148 && (int64_t)c * cbm::size_of_type(type) / (k * 2) >= THREADS * 16 * 8) k *= 2;
