@@ -5,7 +5,7 @@
 // Nothing in these is subtracted that is nearly equal, so a decided row keeps the digits of a log probability near 0.
 // What bounds it is memory: logits are read once, forwards and backwards, and the gradient is written once.  Narrow rows go through shared
 // memory, where lanes of a row lie a bank apart; long ones are gone over once by a block or a cluster, which keeps m, s and t as it goes
-// (2 449 029 x 47 fp32 102 us, 4.5 TB/s, with the gradient 244 us, of 152 at the rate of a copy).
+// (2 449 029 x 47 fp32 102 us, 4.9 TB/s, with the gradient 244 us, of 220 at the rate of a copy).
 // Gradient: dx_j = g_log ([j = label] - p_j) - g_ent p_j (log p_j + entropy) + sum_i g_top_i ([j = c_i] - p_j).
 #include "cbm_common.h"
 #include "cbm_launch.cuh"
@@ -784,8 +784,8 @@ void with_vector(int e, F&& f) {
     }
 }
 
-// Blocks to a row: while the rows alone leave SMs without one (two of them to each), and a part keeps 8 vectors a thread.  (One row of
-// 128 256 fp32: 8 blocks 20.5 us, one 33; 32 rows of 30 000: 16.4, one 20.5.)
+// Blocks to a row: while the rows alone leave SMs without one (two of them to each), and a part keeps 8 vectors a thread.  (16 rows of
+// 128 256 bf16, 20 best: 8 blocks 20.5 us, one 33; 32 rows of 30 000: 16.4, one 20.5.)
 int blocks_to_row(int64_t n, int c, int32_t type) {
     int k = 1;
     while (k < CLUSTER && n * k * 2 <= 2 * 148 && (int64_t)c * cbm::size_of_type(type) / (k * 2) >= THREADS * 16 * 8) k *= 2;
