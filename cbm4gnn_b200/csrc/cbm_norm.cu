@@ -999,8 +999,10 @@ int launched(const char* who) {
     return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
+constexpr int MOST_CHANNELS = 1 << 22;  // (slabs of 128 groups, or of 256 threads, are counted in a grid's second dimension)
+
 int check(const char* who, const Params& p, int32_t type) {
-    const bool fits = p.n_rows >= 0 && p.n_rows < ((int64_t)1 << 40) && p.n_samples >= 0 && p.c >= 1 && p.groups >= 1 && p.c % p.groups == 0 &&
+    const bool fits = p.n_rows >= 0 && p.n_rows < ((int64_t)1 << 40) && p.n_samples >= 0 && p.c >= 1 && p.c <= MOST_CHANNELS && p.groups >= 1 && p.c % p.groups == 0 &&
                       p.ldx >= p.c && p.ldy >= p.c && p.act >= 0 && p.act <= CBM_B200_ACT_SILU && type >= 0 && type <= CBM_B200_FP16 && p.eps >= 0.f &&
                       (p.ptr || (p.rows_each >= 0 && (p.n_samples == 0 ? p.n_rows == 0 : p.n_rows % p.n_samples == 0 && p.n_rows / p.n_samples == p.rows_each)));
     return fits ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes, type or activation");
@@ -1154,7 +1156,7 @@ void launch(Params& p, const Plan& plan, unsigned char* workspace, const cbm::St
             cbm::launch_next(tiles_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
             if (!plan.joins) return;
             joins = p.ptr ? p.tiles : p.n_samples;
-            const int across = p.ptr ? (p.groups < 4 ? p.groups : 4) : p.groups;  // (most blocks of tiles find nothing to do)
+            const int most = p.ptr ? 4 : 65535, across = p.groups < most ? p.groups : most;  // (most blocks of tiles find nothing to do)
             cbm::launch_next(join_kernel<T, GRAD>, dim3((unsigned)((joins + JOINED - 1) / JOINED + (sums ? (p.c + CHANNELS - 1) / CHANNELS : 0)), across), JOINERS, 0, on, p, joins);
             cbm::launch_next(long_kernel<T, E, STRIDED, GRAD>, grid, THREADS, 0, on, p);
         });

@@ -387,7 +387,7 @@ int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int32_t type, 
                                   const float* g_entropy, const float* g_top, void* dx, int64_t lddx, void* stream);
 
 /* cbm_b200_group_norm       y = act(weight (x - mean) / sqrt(var + eps) + bias) for rows x [dev, n_rows x channels] in n_samples
- *                           samples and `groups` equal ranges of channels; mean and variance of each sample's group.  The
+ *                           samples and `groups` equal ranges of channels (up to 2^22 in all); mean and variance of each sample's group.  The
  *                           samples are the rows ptr[s] .. ptr[s + 1] (ptr [dev], n_samples + 1 entries, rising; kept inside the
  *                           rows there are), or rows_each rows each where ptr is NULL.  Rows of no sample get 0.  weight and
  *                           bias [dev, channels], fp32 where wide_params, else of `type`; NULL for 1 and 0.  mean and rstd

@@ -153,3 +153,16 @@ def test_two_captured_graphs_and_an_eager_call_side_by_side():
         last = orthogonalise(us[2])
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(last, want[2])
+
+
+def test_norm_of_more_groups_than_a_grid_is_wide():
+    c = 140_000
+    x = _normal(1, 2, 40, c).bfloat16().requires_grad_(True)
+    gy = _normal(2, 2, 40, c).bfloat16()
+    y = group_norm(x, c // 2)
+    gx, = torch.autograd.grad(y, x, gy)
+    want, bound = norm64(x.detach().reshape(80, c), c // 2, None, None, [0, 40, 80], 1e-5, None, gy.reshape(80, c), y.detach().reshape(80, c))
+    assert_within(y.detach().reshape(80, c), want["y"], bound["y"], "y")
+    assert_within(gx.reshape(80, c), want["gx"], bound["gx"], "gx")
+    with pytest.raises(RuntimeError, match="bad sizes"):
+        group_norm(torch.zeros((2, (1 << 22) + 2), device="cuda"), 2)
