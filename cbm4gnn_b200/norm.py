@@ -132,7 +132,8 @@ def _on_host(x, weight, bias, ptr, samples, rows_each, groups, eps, act):
 def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                ptr: torch.Tensor | None = None, eps: float = 1e-5, activation: str | None = None) -> torch.Tensor:
     """``act(weight * (x - mean) / sqrt(var + eps) + bias)`` with mean and variance of each sample's ``groups`` equal ranges of
-    channels (on the GPU up to 2^22 channels).  ``x``: [N, C], one sample or, with ``ptr``, the samples ``ptr[s] .. ptr[s + 1]``; or [B, n, C], B samples.
+    channels (on the GPU up to 2^22 channels).  ``x``: [N, C], one sample or, with ``ptr``, the samples
+    ``ptr[s] .. ptr[s + 1]``; or [B, n, C], B samples.
     fp32, bf16 or fp16; ``weight`` and ``bias`` [C] of that type or fp32; ``activation`` None, "relu" or "silu".
 
     ``ptr`` (int64 or int32, rising, on x's device; its values are not looked at on the host) may leave samples
