@@ -23,14 +23,16 @@ using u64 = unsigned long long;
 constexpr u32 FULL = 0xffffffffu;
 constexpr float LOWEST = -200.f;  // exp of it is 0: differences are cut off there, so that 0 times infinity does not come up
 
-// Whole numbers in the order of the values: NaN above all, the two zeros equal.
+// Whole numbers in the order of the values: NaN above all, the two zeros equal.  (NaN is not the largest number there is: the key of class 0
+// would then be 2^64 - 1, where the search for the first place starts, and never be behind it.)
+constexpr u32 NAN_KEY = 0xfffffffeu;
 __device__ __forceinline__ u32 ordered(float x) {
-    if (x != x) return 0xffffffffu;
+    if (x != x) return NAN_KEY;
     const u32 b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(u32 key) {
-    return key == 0xffffffffu ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+    return key == NAN_KEY ? NAN : __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 // In the order in which classes are listed: by value, then the lower class first.
 __device__ __forceinline__ u64 key_of(u32 value, u32 j) { return (u64)value << 32 | (u32)~j; }
@@ -641,6 +643,7 @@ __global__ void __launch_bounds__(TILE_THREADS) tile_grad_kernel(const BackwardP
     if (on && !g.closed)
         for (int i = lane; i < p.top; i += p.lanes) {
             const int64_t j = p.top_class[row * p.top + i];
+            if (j < 0 || j >= p.c) continue;  // (no class)
             static_cast<T*>(p.dx)[row * p.ld_out + j] = cbm::narrow<T>(g.base(cbm::widen(static_cast<const T*>(p.x)[row * p.ld + j])) +
                                                                         p.g_top[row * p.top + i] + (j == g.label ? g.gl : 0.f));
         }
@@ -668,6 +671,7 @@ __global__ void __launch_bounds__(256) rows_grad_kernel(const BackwardParams p) 
     if (on && !g.closed)
         for (int i = lane; i < p.top; i += lanes) {
             const int64_t j = p.top_class[row * p.top + i];
+            if (j < 0 || j >= p.c) continue;  // (no class)
             dx[j] = cbm::narrow<T>(g.base(cbm::widen(x[j])) + p.g_top[row * p.top + i] + (j == g.label ? g.gl : 0.f));
         }
 }
