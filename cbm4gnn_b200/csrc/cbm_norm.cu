@@ -12,9 +12,9 @@
 //   * Longer samples: every tile leaves a partial result, a warp or a block to a sample joins them in a fixed order, and a third kernel
 //     goes over the rows again, from their ends, which L2 still holds.
 //   * A few samples of some hundred rows: a cluster of blocks to each, which join through one another's shared memory: one launch.
-//   * Groups wider than a block's threads hold: a block to each, value by value.
-// Means and squares around them are kept for every few rows and joined (mean and sum of squares around it of two parts give those of
-// both), so that a mean far from 0 costs no digits; no sum depends on the order in which blocks run.
+//   * Groups wider than a block's threads hold: a block to each, value by value, with sums in 64 bits.
+// Elsewhere means and squares around them are kept for every few rows and joined (mean and sum of squares around it of two parts give those
+// of both), so that a mean far from 0 costs no digits; no sum depends on the order in which blocks run.
 #include "cbm_common.h"
 #include "cbm_launch.cuh"
 #include "cbm_values.cuh"
@@ -896,13 +896,14 @@ __global__ void __launch_bounds__(THREADS, blocks_resident(E, GRAD)) cluster_ker
 }
 
 // ---- groups that are wider than a block -----------------------------------------------------------
-__device__ __forceinline__ float block_sum(float v) {
-    __shared__ float part[THREADS / 32];
-    v = lanes_sum(v, 32);
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[THREADS / 32];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.f;
+    double s = 0.0;
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) s += part[i];
     return s;
@@ -914,7 +915,8 @@ __device__ __forceinline__ float slope_by(float z, int act) {
     return s;
 }
 
-// A block to a sample's group, value by value.
+// A block to a sample's group, value by value.  A thread adds up to rows x width / 256 values: in 64 bits, as in 32 the sum of a long
+// sample far from 0 is off by more than its spread (50 000 x 4 096 around 1 000: the mean by five spreads, the variance 27 times).
 template <class T, bool GRAD>
 __global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
     cbm::wait_before();
@@ -922,18 +924,18 @@ __global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
         const int64_t s = unit / p.groups, first = start_of(p, s), last = max(start_of(p, s + 1), first), count = (last - first) * p.width;
         const int c0 = (int)(unit % p.groups) * p.width;
         const T *x = static_cast<const T*>(p.x), *gy = static_cast<const T*>(p.gy);
-        const float share = 1.f / (float)max(count, (int64_t)1);
+        const double share = 1.0 / (double)max(count, (int64_t)1);
         // f(row, channel, value)
         auto each = [&](auto&& f) {
             for (int64_t row = first; row < last; ++row)
                 for (int c = threadIdx.x; c < p.width; c += THREADS) f(row, c0 + c, cbm::widen(x[row * p.ldx + c0 + c]));
         };
-        float sum = 0.f;
+        double sum = 0.0;
         each([&](int64_t, int, float v) { sum += v; });
-        const float mean = block_sum(sum) * share;
-        sum = 0.f;
+        const float mean = (float)(block_sum(sum) * share);
+        sum = 0.0;
         each([&](int64_t, int, float v) { sum += (v - mean) * (v - mean); });
-        const float r = rsqrtf(block_sum(sum) * share + p.eps);
+        const float r = rsqrtf((float)(block_sum(sum) * share) + p.eps);
         if constexpr (!GRAD) {
             each([&](int64_t row, int c, float v) {
                 const float z = (v - mean) * (r * param<T>(p.w, p.wide_params, c, 1.f)) + param<T>(p.b, p.wide_params, c, 0.f);
@@ -941,16 +943,16 @@ __global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
             });
             if (threadIdx.x == 0 && p.mean) p.mean[unit] = mean, p.r[unit] = r;
         } else {
-            float su = 0.f, sux = 0.f;
+            double all_u = 0.0, all_ux = 0.0;
             auto u_of = [&](int64_t row, int c, float xh) {
                 const float w = param<T>(p.w, p.wide_params, c, 1.f);
                 return cbm::widen(gy[row * p.ldgy + c]) * slope_by(xh * w + param<T>(p.b, p.wide_params, c, 0.f), p.act) * w;
             };
             each([&](int64_t row, int c, float v) {
                 const float xh = (v - mean) * r, u = u_of(row, c, xh);
-                su += u, sux += u * xh;
+                all_u += u, all_ux += u * xh;
             });
-            su = block_sum(su) * share, sux = block_sum(sux) * share;
+            const float su = (float)(block_sum(all_u) * share), sux = (float)(block_sum(all_ux) * share);
             each([&](int64_t row, int c, float v) {
                 const float xh = (v - mean) * r;
                 static_cast<T*>(p.y)[row * p.ldy + c] = cbm::narrow<T>(r * (u_of(row, c, xh) - su - xh * sux));
@@ -960,14 +962,14 @@ __global__ void __launch_bounds__(THREADS) wide_kernel(const Params p) {
     }
 }
 
-// Sums over ranges of rows of g xh and g, a thread to a channel; behind wide_kernel, with its statistics.
+// Sums over ranges of samples of g xh and g, a thread to a channel, in 64 bits like those above; behind wide_kernel, with its statistics.
 template <class T>
 __global__ void __launch_bounds__(THREADS) wide_params_kernel(const Params p) {
     cbm::wait_before();
     const int c = blockIdx.y * THREADS + threadIdx.x;
     if (c >= p.c) return;
     const float w = param<T>(p.w, p.wide_params, c, 1.f), b = param<T>(p.b, p.wide_params, c, 0.f);
-    float2 all{0.f, 0.f};
+    double all_x = 0.0, all = 0.0;
     const int64_t each = (p.n_samples + p.parts - 1) / p.parts, to = min((blockIdx.x + 1) * each, p.n_samples);
     for (int64_t s = blockIdx.x * each; s < to; ++s) {
         const float2 at = p.joined[s * p.groups + c / p.width];
@@ -975,10 +977,10 @@ __global__ void __launch_bounds__(THREADS) wide_params_kernel(const Params p) {
         for (int64_t row = start_of(p, s); row < last; ++row) {
             const float xh = (cbm::widen(static_cast<const T*>(p.x)[row * p.ldx + c]) - at.x) * at.y;
             const float g = cbm::widen(static_cast<const T*>(p.gy)[row * p.ldgy + c]) * slope_by(xh * w + b, p.act);
-            all.x += g * xh, all.y += g;
+            all_x += g * xh, all += g;
         }
     }
-    p.channels[(int64_t)blockIdx.x * p.c + c] = all;
+    p.channels[(int64_t)blockIdx.x * p.c + c] = float2{(float)all_x, (float)all};
 }
 
 // Rows of no sample: 0.

@@ -3,8 +3,9 @@ import pytest
 import torch
 
 from cbm4gnn_b200.classify import class_log_probs
+from cbm4gnn_b200.norm import group_norm
 
-from operators64 import assert_within, classes64
+from operators64 import SUM, U, assert_within, classes64, half_step, norm64, smallest
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -43,3 +44,50 @@ def test_undefined_classes_are_listed_like_others(kind, c, top):
         assert_within(r.top_log_probs.detach(), want["top"], bound["top"], "top")
         gx, = torch.autograd.grad(r.top_log_probs, x, gt)
         assert_within(gx, want["gx"], bound["gx"], "gx")
+
+
+# --------------------------------------------------------------------------------- groups wider than a block
+def _check_norm(x, groups, ptr, activation, kind=None, close=False):
+    """``close``: of a mean far from 0 no more may be lost than its one rounding, and that of x - mean."""
+    c = x.size(-1)
+    leaves = [t.to(kind or x.dtype).requires_grad_(True) for t in (_normal(1, c) + 1, _normal(2, c))]
+    x = x.detach().requires_grad_(True)
+    gy = _normal(3, *x.shape).to(x.dtype)
+    on = None if ptr is None or x.dim() == 3 else torch.tensor(ptr, device="cuda")
+    y = group_norm(x, groups, *leaves, ptr=on, activation=activation)
+    got = dict(zip(("gx", "gw", "gb"), torch.autograd.grad(y, (x, *leaves), gy)))
+    n = x.numel() // c
+    flat = x.detach().reshape(n, c)
+    rows = ptr or [0, n]
+    want, bound = norm64(flat, groups, *leaves, rows, 1e-5, activation, gy.reshape(n, c), y.detach().reshape(n, c))
+    assert_within(y.detach().reshape(n, c), want["y"], bound["y"], "y")
+    assert_within(got["gx"].reshape(n, c), want["gx"], bound["gx"], "gx")
+    for k in ("gw", "gb"):  # (rounded to the parameter's type: half a step of the value, 2^-25 below the normal numbers of fp16)
+        assert_within(got[k], want[k], bound[k] + half_step(got[k].dtype) * want[k].abs() + smallest(got[k].dtype), k)
+    if close:
+        assert activation is None and rows == [0, n] and x.dtype == torch.float32
+        v = flat.double().view(n, groups, -1)
+        mean, r = v.mean((0, 2), keepdim=True), (v.var((0, 2), keepdim=True, correction=0) + 1e-5).rsqrt()
+        w, b = (t.detach().double().view(1, groups, -1) for t in leaves)
+        xh = (v - mean) * r
+        near = w.abs() * (r * 2 * U * mean.abs() + (SUM + 8 * U) * xh.abs()) + 4 * U * ((xh * w + b).abs() + b.abs())
+        assert_within(y.detach().view(n, groups, -1), xh * w + b, near, "y beside a large mean")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,c,groups,ptr", [
+    (1, 2049, 1, None), (300, 2049, 1, None), (150, 4100, 2, None), (90, 8200, 2, None), (40, 12_300, 3, [0, 0, 7, 7, 30, 40]), (64, 4096, 1, [3, 20, 20, 50]),
+    (30, 2051, 1, [30, 30]), (30, 2500, 1, [0, 0]), (33, 9000, 1, list(range(34)))])
+def test_norm_of_wide_groups(kind, n, c, groups, ptr):
+    _check_norm((_normal(n, n, c) * 1.5 + 0.4).to(kind), groups, ptr, "silu", kind)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("b,n,c,groups", [(50, 1, 1100, 1), (37, 1, 4096, 1), (9, 1, 8200, 2), (7, 1, 9000, 1), (5, 1, 4095, 1), (6, 9, 4100, 1), (3, 20, 5000, 2)])
+def test_norm_of_equal_samples_of_wide_groups(kind, b, n, c, groups):
+    _check_norm((_normal(b, b, n, c) - 0.7).to(kind), groups, list(range(0, b * n + 1, n)), "relu")
+
+
+@pytest.mark.parametrize("n,c,groups,mean", [(6000, 4096, 1, 1000.0), (10_000, 2304, 1, 100.0), (3000, 5000, 2, -3.0)])
+def test_norm_of_wide_groups_keeps_digits_beside_a_large_mean(n, c, groups, mean):
+    _check_norm(mean + _normal(5, n, c), groups, None, None, close=True)
