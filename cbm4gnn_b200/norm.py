@@ -107,7 +107,7 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def _on_host(x, weight, bias, ptr, samples, rows_each, groups, eps, act):
-    """The same by torch's elementary operations, for CPU tensors."""
+    """The same by torch's elementary operations, for CPU tensors; a sample's rows are added up in 64 bits."""
     n, c = x.shape
     v = x.float()
     if ptr is None:
@@ -118,8 +118,9 @@ def _on_host(x, weight, bias, ptr, samples, rows_each, groups, eps, act):
     size = (torch.bincount(row, minlength=samples + 1) * (c // groups)).clamp_min(1)[:, None]
 
     def mean(t):
-        of_row = t.reshape(n, groups, c // groups).sum(2)
-        return (of_row.new_zeros((samples + 1, groups)).index_add(0, row, of_row) / size)[row].repeat_interleave(c // groups, dim=1)
+        of_row = t.reshape(n, groups, c // groups).sum(2, dtype=torch.float64)
+        of_sample = of_row.new_zeros((samples + 1, groups)).index_add(0, row, of_row) / size
+        return of_sample[row].float().repeat_interleave(c // groups, dim=1)
 
     d = v - mean(v)
     z = d * torch.rsqrt(mean(d * d) + eps)
