@@ -115,6 +115,7 @@ def _on_host(x, weight, bias, ptr, samples, rows_each, groups, eps, act):
     else:
         row = torch.bucketize(torch.arange(n), ptr[1:].contiguous(), right=True)
         row = torch.where((row >= samples) | (torch.arange(n) < (ptr[0] if samples else 0)), samples, row)
+        v = torch.where((row < samples)[:, None], v, 0.0)  # (whatever rows of no sample hold does not come into sums of gradients)
     size = (torch.bincount(row, minlength=samples + 1) * (c // groups)).clamp_min(1)[:, None]
 
     def mean(t):

@@ -91,3 +91,21 @@ def test_norm_of_equal_samples_of_wide_groups(kind, b, n, c, groups):
 @pytest.mark.parametrize("n,c,groups,mean", [(6000, 4096, 1, 1000.0), (10_000, 2304, 1, 100.0), (3000, 5000, 2, -3.0)])
 def test_norm_of_wide_groups_keeps_digits_beside_a_large_mean(n, c, groups, mean):
     _check_norm(mean + _normal(5, n, c), groups, None, None, close=True)
+
+
+@pytest.mark.parametrize("n,c,groups,ptr", [(40, 24, 6, [3, 10, 10, 30]), (5000, 64, 8, [100, 4000, 4010, 4500]), (60, 2500, 1, [2, 30, 50])])
+def test_norm_rows_of_no_sample_may_hold_anything(n, c, groups, ptr):
+    x = _normal(1, n, c)
+    x[:ptr[0]], x[ptr[-1]:] = torch.nan, torch.inf
+    clean = x.clone()
+    clean[:ptr[0]] = clean[ptr[-1]:] = 0.0
+    on, gy = torch.tensor(ptr, device="cuda"), _normal(4, n, c)
+    found = []
+    for t in (x, clean):
+        leaves = [t.requires_grad_(True), _normal(2, c).requires_grad_(True), _normal(3, c).requires_grad_(True)]
+        y = group_norm(leaves[0], groups, *leaves[1:], ptr=on, activation="silu")
+        found.append((y.detach(), *torch.autograd.grad(y, leaves, gy)))
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
+    for t in found[0][:2]:
+        assert t[:ptr[0]].eq(0).all() and t[ptr[-1]:].eq(0).all()
