@@ -1224,7 +1224,7 @@ extern "C" int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* 
     if (ldgy < channels) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: rows of the gradient overlap");
     if (n_rows && (!x || !gy || !gx)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
     const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), true);
-    if (n_rows && (plan.way == TILES || plan.way == CLUSTERS) && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
+    if (n_rows && n_samples && (plan.way == TILES || plan.way == CLUSTERS) && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
     const int64_t need = plan.bytes(n_samples, channels, groups, true);
     if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: workspace too small");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));

@@ -109,3 +109,12 @@ def test_norm_rows_of_no_sample_may_hold_anything(n, c, groups, ptr):
         assert torch.equal(a, b)
     for t in found[0][:2]:
         assert t[:ptr[0]].eq(0).all() and t[ptr[-1]:].eq(0).all()
+
+
+@pytest.mark.parametrize("n,c,groups", [(9, 12, 4), (3000, 64, 8), (40, 2500, 1)])
+def test_norm_of_rows_without_samples(n, c, groups):
+    """A list of no graphs: no row belongs to one."""
+    x, w, b = (t.requires_grad_(True) for t in (_normal(1, n, c), _normal(2, c), _normal(3, c)))
+    y = group_norm(x, groups, w, b, ptr=torch.zeros(1, dtype=torch.int64, device="cuda"), activation="silu")
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), _normal(4, n, c))
+    assert y.shape == x.shape and all(t.eq(0).all() for t in (y, gx, gw, gb))
