@@ -118,3 +118,37 @@ def test_norm_of_rows_without_samples(n, c, groups):
     y = group_norm(x, groups, w, b, ptr=torch.zeros(1, dtype=torch.int64, device="cuda"), activation="silu")
     gx, gw, gb = torch.autograd.grad(y, (x, w, b), _normal(4, n, c))
     assert y.shape == x.shape and all(t.eq(0).all() for t in (y, gx, gw, gb))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("c,top", [(2, 1), (7, 3), (47, 0), (200, 2), (600, 5), (1300, 3), (20_000, 4)])
+@pytest.mark.parametrize("grads", [(True, False, False), (True, True, True), (False, False, True)])
+def test_gradients_of_decided_rows_keep_their_digits(kind, c, top, grads):
+    """Where one class has all but 1e-9 to 1e-3 of a row, what is left of its own gradient is a product with 1 - p, not a difference."""
+    n = 16
+    lead = torch.linspace(7.0, 20.0, n, device="cuda") + torch.tensor(float(c)).log().cuda()
+    lead = lead.clamp_max(27.0)
+    for pitch, first in ((c, 0), (c + 3, 1)):
+        wide = torch.zeros((n, pitch), dtype=kind, device="cuda")
+        wide[:, first:first + c] = (0.5 * _normal(c, n, c)).to(kind)
+        x = wide[:, first:first + c]
+        labels = torch.arange(n, device="cuda") * 7 % c
+        x[torch.arange(n), labels] = lead.to(kind)
+        x = x.detach().requires_grad_(True)
+        given = [_normal(9 + i, *s) if on and s[-1] else None for i, (on, s) in enumerate(zip(grads, ((n,), (n,), (n, top))))]
+        r = class_log_probs(x, labels, top=top)
+        used = [(o, g) for o, g in zip(r[:3], given) if g is not None]
+        if not used:
+            continue
+        gx, = torch.autograd.grad([o for o, _ in used], x, [g for _, g in used])
+        want, bound = classes64(x, labels, top, *given)
+        # terms of 1 - p: arguments of up to 30 rounded once, exp's 2 steps and as many of its own argument, the sum, some operations more
+        d = x.detach().double() - x.detach().double().gather(1, labels[:, None])
+        left = torch.exp(d).scatter(1, labels[:, None], 0.0).sum(1)
+        left, own = left / (1 + left), labels[:, None]
+        zero = torch.zeros(n, dtype=torch.float64, device="cuda")
+        gl, ge = (zero if g is None else g.double() for g in given[:2])
+        gt = zero[:, None] if given[2] is None else given[2].double()
+        near = (SUM + 128 * U) * (gl.abs() * left + gt[:, 0].abs() * left + ge.abs() * (want["entropy"] + left)) + 8 * U * gt[:, 1:].abs().sum(1)
+        near = near + 2 * half_step(kind) * want["gx"].gather(1, own)[:, 0].abs() + smallest(kind)
+        assert_within(gx, want["gx"], bound["gx"].scatter(1, own, near[:, None]), "gx")
