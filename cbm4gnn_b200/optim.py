@@ -102,7 +102,7 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
                 g = g.contiguous()
                 held.append(g)
             for t in (w, m):
-                if t.numel() and (t.stride(1) != 1 or (t.size(0) > 1 and t.stride(0) < t.size(1))):
+                if t.numel() and ((t.size(1) > 1 and t.stride(1) != 1) or (t.size(0) > 1 and t.stride(0) < t.size(1))):
                     raise RuntimeError("orthogonal step: weights and momenta of unit column stride expected")
             rows, cols = w.shape
             words.extend((w.data_ptr(), g.data_ptr(), m.data_ptr(), *(max(t.stride(0), cols) for t in (w, g, m)), rows | cols << 32))

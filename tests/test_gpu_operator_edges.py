@@ -4,8 +4,9 @@ import torch
 
 from cbm4gnn_b200.classify import class_log_probs
 from cbm4gnn_b200.norm import group_norm
+from cbm4gnn_b200.optim import OrthogonalSGD, orthogonal_step, orthogonalise
 
-from operators64 import SUM, U, assert_within, classes64, half_step, norm64, smallest
+from operators64 import SUM, U, assert_within, classes64, half_step, norm64, ortho64, smallest
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -152,3 +153,25 @@ def test_gradients_of_decided_rows_keep_their_digits(kind, c, top, grads):
         near = (SUM + 128 * U) * (gl.abs() * left + gt[:, 0].abs() * left + ge.abs() * (want["entropy"] + left)) + 8 * U * gt[:, 1:].abs().sum(1)
         near = near + 2 * half_step(kind) * want["gx"].gather(1, own)[:, 0].abs() + smallest(kind)
         assert_within(gx, want["gx"], bound["gx"].scatter(1, own, near[:, None]), "gx")
+
+
+# ------------------------------------------------------------------------------------------------- update
+def test_step_of_a_turned_row():
+    """A weight of one column may have any column stride: torch calls it contiguous, whatever it was made from."""
+    for m in (5, 300):
+        w, g, mom = (_normal(i, 1, m).t() for i in range(3))
+        assert w.stride() == (1, m) and w.is_contiguous()
+        m1 = 0.9 * mom.double() + g.double()
+        o, bound = ortho64(g.double() + 0.9 * m1, 5)
+        want = w.double() - 0.1 * m ** 0.5 * o
+        orthogonal_step([w], [g], [mom], lr=0.1, momentum=0.9)
+        assert (w.double() - want).norm() <= 0.1 * m ** 0.5 * bound + 2.0 ** -23 * want.norm()
+        assert torch.allclose(mom.double(), m1, atol=1e-6, rtol=1e-6)
+        assert (orthogonalise(g).double() - ortho64(g, 5)[0]).norm() <= ortho64(g, 5)[1]
+    p = torch.nn.Parameter(_normal(7, 1, 40).t())
+    p.grad = _normal(8, 40, 1)
+    before = p.detach().clone()
+    OrthogonalSGD([p], lr=0.1).step()
+    assert (p.detach() - before).norm() > 0.1
+    with pytest.raises(RuntimeError, match="unit column stride"):
+        orthogonal_step([_normal(1, 6, 4).t()], [_normal(2, 4, 6)], [_normal(3, 4, 6)], lr=0.1)
