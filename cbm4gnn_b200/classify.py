@@ -13,7 +13,8 @@ import torch
 from .dense import _call, _ld, _rows
 from .norm import TYPES, _data, needs_function, only_once, rows_like
 
-MAX_TOP = 32  # include/cbm_b200.h, CBM_B200_MAX_TOP
+MAX_TOP = 32           # include/cbm_b200.h, CBM_B200_MAX_TOP
+MAX_CLASSES = 1 << 30  # on the GPU
 
 
 class ClassLogProbs(NamedTuple):
@@ -79,11 +80,12 @@ def _on_host(logits, labels, top):
 
 def class_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0) -> ClassLogProbs:
     """For every row of ``logits`` [N, C] (fp32, bf16 or fp16; rows at any pitch): the log probability of its class
-    ``labels`` [N] (int64 or int32), the entropy of the row and its ``top`` most probable classes (0 to 32).
+    ``labels`` [N] (int64 or int32), the entropy of the row and its ``top`` most probable classes (0 to 32).  On the GPU up to
+    2^31 - 1 rows and 2^30 classes; rows of more than 1 024 classes up to 2^31 - 1 stretches of 4 096.
 
     A negative label stands for none: log probability 0, no gradient.  One of C or more gives NaN.  A logit of -inf closes a
     class; a row without an open class has log probabilities -inf, entropy 0 and no gradient.  A row with NaN or +inf is
-    NaN throughout.  Differentiable once in ``logits``, through all three results.
+    NaN throughout, and its gradient is, with a label or without.  Differentiable once in ``logits``, through all three results.
     """
     shape = logits.shape
     if len(shape) != 2 or shape[1] < 1 or labels.shape != shape[:1]:
@@ -98,6 +100,8 @@ def class_log_probs(logits: torch.Tensor, labels: torch.Tensor, top: int = 0) ->
         raise ValueError(f"top must be between 0 and {min(MAX_TOP, shape[1])}")
     if not logits.is_cuda:
         return _on_host(logits, labels, top)
+    if shape[1] > MAX_CLASSES:  # (asked here: the library's sizes have 32 bits)
+        raise RuntimeError(f"class log probabilities: {shape[1]} classes, at most {MAX_CLASSES} on the GPU")
     x, labels = _rows(logits), labels.contiguous()
     if needs_function(x):
         return ClassLogProbs(*_ClassLogProbs.apply(x, labels, int(top)))

@@ -743,8 +743,10 @@ __global__ void __launch_bounds__(THREADS) long_grad_kernel(const BackwardParams
 
 constexpr int ROW_MAX = 1024;  // classes that 32 lanes hold in registers, 32 each
 
+constexpr int MOST_CLASSES = 1 << 30;  // (sums of an index and a stretch's classes are held in 31 bits)
+
 int check(const char* who, int64_t n, int64_t ld, int32_t c, int32_t top, int32_t type) {
-    if (n < 0 || c < 1 || ld < c || top < 0 || top > CBM_B200_MAX_TOP || top > c || type < 0 || type > CBM_B200_FP16)
+    if (n < 0 || c < 1 || c > MOST_CLASSES || ld < c || top < 0 || top > CBM_B200_MAX_TOP || top > c || type < 0 || type > CBM_B200_FP16)
         return cbm::fail(CBM_B200_ERR_ARG, std::string(who) + ": bad sizes or type");
     // (a grid has at most 2^31 - 1 blocks: a row to 32 lanes, or to a block for every stretch of 4 096 classes)
     if (n > ((int64_t)1 << 31) - 1 || (c > ROW_MAX && n * ((c + 4095) / 4096) > ((int64_t)1 << 31) - 1))

@@ -19,6 +19,7 @@ from .dense import _call, _ld, _rows
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # CBM_B200_FP32, ...
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}                      # CBM_B200_ACT_NONE, ...
+MAX_CHANNELS = 1 << 22                                             # on the GPU
 
 
 def rows_like(x: torch.Tensor) -> torch.Tensor:
@@ -179,6 +180,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
         samples, rows_each, rows = 1, shape[0], x
     if not x.is_cuda:
         return _on_host(rows, weight, bias, ptr, samples, rows_each, groups, eps, act).view(shape)
+    if c > MAX_CHANNELS:  # (asked here: the library's sizes have 32 bits)
+        raise RuntimeError(f"group norm: bad sizes, {c} channels, at most {MAX_CHANNELS} on the GPU")
     rows = _rows(rows)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
     sizes = (samples, rows_each, groups, float(eps), act, wide)

@@ -16,7 +16,8 @@ from . import _lib
 from .dense import _call
 
 QUINTIC = (3.4445, -4.7750, 2.0315)
-MAX_STEPS = 64  # include/cbm_b200.h, CBM_B200_MAX_STEPS
+MAX_STEPS = 64                          # include/cbm_b200.h, CBM_B200_MAX_STEPS
+MAX_SIDE, MAX_STACK = 1 << 16, 1 << 15  # on the GPU
 
 
 def _on_host(u, steps, eps):
@@ -38,10 +39,15 @@ def _check_steps(steps, eps):
         raise ValueError("eps must not be negative")
 
 
+def _too_large(rows, cols):
+    return f"{rows} x {cols}, sides of at most {MAX_SIDE} on the GPU" if max(rows, cols) > MAX_SIDE else None
+
+
 def orthogonalise(update: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> torch.Tensor:
     """``update`` [m, n] or [B, m, n] (fp32; each matrix for itself) divided by its norm plus ``eps`` and led towards the
     nearest matrix with orthonormal rows or columns by ``steps`` quintic Newton-Schulz products: five take singular values from
-    a few thousandths of the norm up to between 0.68 and 1.21.  A matrix of zeros stays one.  Not differentiable."""
+    a few thousandths of the norm up to between 0.68 and 1.21.  A matrix of zeros stays one.  Not differentiable.
+    On the GPU sides of up to 65 536 and stacks of up to 32 768."""
     if update.dim() not in (2, 3):
         raise RuntimeError(f"orthogonalise: [m, n] or [B, m, n] expected, not {tuple(update.shape)}")
     if update.dtype != torch.float32:
@@ -52,6 +58,8 @@ def orthogonalise(update: torch.Tensor, steps: int = 5, eps: float = 1e-7) -> to
         return torch.empty_like(u)
     if not u.is_cuda:
         return _on_host(u, steps, eps)
+    if _too_large(u.size(-2), u.size(-1)) or (u.dim() == 3 and u.size(0) > MAX_STACK):  # (asked here: the library's sizes have 32 bits)
+        raise RuntimeError(f"orthogonalise: {tuple(u.shape)}, sides of at most {MAX_SIDE} and stacks of at most {MAX_STACK} on the GPU")
     if u.stride(-1) != 1 or u.stride(-2) < u.size(-1):
         u = u.contiguous()
     batch, rows, cols = (1, *u.shape) if u.dim() == 2 else u.shape
@@ -70,7 +78,8 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
         m <- momentum m + g;  u = g + momentum m (nesterov) or m
         w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalise(u, steps, eps)
 
-    All tensors of a call lie on one device; weights and momenta must not overlap one another or the gradients."""
+    All tensors of a call lie on one device; weights and momenta must not overlap one another or the gradients.  On the GPU
+    sides of up to 65 536."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
         raise RuntimeError(f"orthogonal step: {len(weights)} weights, {len(grads)} gradients, {len(momenta)} momenta")
@@ -105,6 +114,8 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
                 if t.numel() and ((t.size(1) > 1 and t.stride(1) != 1) or (t.size(0) > 1 and t.stride(0) < t.size(1))):
                     raise RuntimeError("orthogonal step: weights and momenta of unit column stride expected")
             rows, cols = w.shape
+            if _too_large(rows, cols):
+                raise RuntimeError(f"orthogonal step: {_too_large(rows, cols)}")
             words.extend((w.data_ptr(), g.data_ptr(), m.data_ptr(), *(max(t.stride(0), cols) for t in (w, g, m)), rows | cols << 32))
         of = words.buffer_info()[0]
         space = _lib.lib().cbm_b200_orthogonal_step_workspace(of, len(weights))
@@ -115,7 +126,8 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
 
 
 class OrthogonalSGD(torch.optim.Optimizer):
-    """``orthogonal_step`` on the weights of dense maps.  Takes matrices alone: biases and norms go to another optimiser."""
+    """``orthogonal_step`` on the weights of dense maps.  Takes matrices alone, on the GPU with sides of up to 65 536: biases, norms and
+    the embeddings of a large graph's nodes go to another optimiser."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  eps: float = 1e-7):
@@ -129,6 +141,8 @@ class OrthogonalSGD(torch.optim.Optimizer):
         for p in self.param_groups[-1]["params"]:
             if p.dim() != 2 or p.dtype != torch.float32:
                 raise ValueError(f"OrthogonalSGD updates fp32 matrices, not {p.dtype} of {tuple(p.shape)}")
+            if p.is_cuda and _too_large(*p.shape):
+                raise ValueError(f"OrthogonalSGD: {_too_large(*p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -366,7 +366,8 @@ int cbm_b200_spmm_update_static(cbm_b200_plan* p, const float* x, int64_t ldx, f
  *
  * cbm_b200_class_log_probs       for every row of logits [dev, n_rows x n_classes, leading dimension ld]: the log
  *                                probability of its label, the entropy of the row, and its `top` most probable
- *                                classes with their log probabilities (equal logits: lower class first; top <= n_classes).
+ *                                classes with their log probabilities (equal logits: lower class first; top <= n_classes; up to 2^30
+ *                                classes).
  *                                labels [dev]: int64 where wide_labels, else int32; negative: none (log probability 0);
  *                                n_classes or more: NaN.  stats [dev, 2 x n_rows, 8-byte aligned] is for the gradient, or NULL.
  *                                top_log_prob, top_class [dev, n_rows x top].

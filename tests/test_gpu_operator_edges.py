@@ -175,3 +175,32 @@ def test_step_of_a_turned_row():
     assert (p.detach() - before).norm() > 0.1
     with pytest.raises(RuntimeError, match="unit column stride"):
         orthogonal_step([_normal(1, 6, 4).t()], [_normal(2, 4, 6)], [_normal(3, 4, 6)], lr=0.1)
+
+
+# ------------------------------------------------------------------------------------------------- limits
+def test_sizes_past_the_limits_are_refused_by_name():
+    """Before anything is copied or counted in 32 bits; the operands are broadcasts of one value."""
+    one = torch.ones((1, 1), device="cuda")
+    labels = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for c in ((1 << 22) + 4, (1 << 32) + 4):
+        with pytest.raises(RuntimeError, match=f"{c} channels, at most {1 << 22}"):
+            group_norm(one.expand(1, c), 2)
+        with pytest.raises(RuntimeError, match=f"{c} channels, at most {1 << 22}"):
+            group_norm(one.expand(1, c), 2, ptr=labels)
+    for c in ((1 << 30) + 1, (1 << 32) + 4):
+        with pytest.raises(RuntimeError, match=f"{c} classes, at most {1 << 30}"):
+            class_log_probs(one.expand(1, c), labels)
+    for m, n in ((65_537, 3), (3, 65_537), ((1 << 32) + 5, 7), (7, (1 << 32) + 5)):
+        with pytest.raises(RuntimeError, match="65536"):
+            orthogonalise(one.expand(m, n))
+        with pytest.raises(ValueError, match=f"{m} x {n}, sides of at most 65536"):
+            OrthogonalSGD([torch.nn.Parameter(one.expand(m, n))])
+    with pytest.raises(RuntimeError, match="stacks of at most 32768"):
+        orthogonalise(one.expand(32_769, 2, 2))
+    w, fine = torch.zeros((65_537, 2), device="cuda"), torch.ones((4, 4), device="cuda")
+    with pytest.raises(RuntimeError, match="65537 x 2"):
+        orthogonal_step([fine, w], [fine.clone(), w.clone()], [torch.zeros_like(fine), w.clone()], lr=0.1)
+    assert fine.eq(1).all()
+    tall = _normal(1, 65_536, 2)
+    want, bound = ortho64(tall, 5)
+    assert (orthogonalise(tall).double() - want).norm() <= bound
