@@ -838,6 +838,7 @@ extern "C" int cbm_b200_class_log_probs(const void* logits, int64_t ld, int32_t 
     if (n_rows == 0) return CBM_B200_OK;
     if (!logits || !labels || !log_prob || !entropy || (top && (!top_log_prob || !top_class)))
         return cbm::fail(CBM_B200_ERR_ARG, "class_log_probs: NULL argument");
+    if (reinterpret_cast<uintptr_t>(stats) % 8) return cbm::fail(CBM_B200_ERR_ARG, "class_log_probs: statistics not at 8 bytes");
     ForwardParams p{logits, labels, ld, n_rows, n_classes, top, wide_labels, 1, 0, log_prob, entropy, stats, top_log_prob, top_class};
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
     cbm::with_type(type, [&](auto t) {
@@ -876,6 +877,7 @@ extern "C" int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int
     if (n_rows == 0) return CBM_B200_OK;
     if (!logits || !labels || !stats || !entropy || !dx || (g_top && top && !top_class))
         return cbm::fail(CBM_B200_ERR_ARG, "class_log_probs_grad: NULL argument");
+    if (reinterpret_cast<uintptr_t>(stats) % 8) return cbm::fail(CBM_B200_ERR_ARG, "class_log_probs_grad: statistics not at 8 bytes");
     BackwardParams p{logits, labels, ld, lddx, n_rows, n_classes, top, wide_labels, 1, 0, stats, entropy, g_log_prob, g_entropy, g_top, top_class, dx};
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
     cbm::with_type(type, [&](auto t) {

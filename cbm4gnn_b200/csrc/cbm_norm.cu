@@ -1205,7 +1205,8 @@ extern "C" int cbm_b200_group_norm(const void* x, int64_t ldx, int32_t type, int
     if (!x || !y || !mean != !rstd) return cbm::fail(CBM_B200_ERR_ARG, "group_norm: NULL argument");
     const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), false);
     const int64_t need = plan.bytes(n_samples, channels, groups, false);
-    if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm: workspace too small");
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+        return cbm::fail(CBM_B200_ERR_ARG, "group_norm: workspace too small, or not at 8 bytes");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
     cbm::with_type(type, [&](auto t) { launch<decltype(t), false>(p, plan, static_cast<unsigned char*>(workspace), on); });
     return launched("group_norm");
@@ -1226,7 +1227,8 @@ extern "C" int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* 
     const Plan plan(n_rows, n_samples, ptr != nullptr, rows_each, channels, groups, form_of(p, cbm::size_of_type(type)), true);
     if (n_rows && n_samples && (plan.way == TILES || plan.way == CLUSTERS) && (!mean || !rstd)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: NULL argument");
     const int64_t need = plan.bytes(n_samples, channels, groups, true);
-    if (need && (!workspace || workspace_bytes < need)) return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: workspace too small");
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+        return cbm::fail(CBM_B200_ERR_ARG, "group_norm_grad: workspace too small, or not at 8 bytes");
     const cbm::Stream on(static_cast<cudaStream_t>(stream));
     cbm::with_type(type, [&](auto t) { launch<decltype(t), true>(p, plan, static_cast<unsigned char*>(workspace), on); });
     return launched("group_norm_grad");

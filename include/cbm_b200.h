@@ -395,7 +395,7 @@ int cbm_b200_class_log_probs_grad(const void* logits, int64_t ld, int32_t type, 
  *                           [dev, n_samples x groups] for the gradient, both NULL where none follows.  (Where samples are one row
  *                           each, the gradient does without them: not written and not read.)
  * cbm_b200_group_norm_grad  gx, and gw and gb [dev, channels] (NULL: not wanted).
- * cbm_b200_group_norm_workspace  bytes of workspace [dev] of either (`gradient` 0 or 1); n_samples negative: without ptr. */
+ * cbm_b200_group_norm_workspace  bytes of workspace [dev, 8-byte aligned] of either (`gradient` 0 or 1); n_samples negative: without ptr. */
 #define CBM_B200_ACT_NONE 0
 #define CBM_B200_ACT_RELU 1
 #define CBM_B200_ACT_SILU 2
