@@ -70,7 +70,7 @@ int check_timeout(const char* who) {
     if (!w) return cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": no usable CUDA device on this thread");
     if (*(volatile int*)w) {
         *(volatile int*)w = 0;
-        return cbm::fail(CBM_B200_ERR_TIMEOUT, std::string(who) + ": a bounded wait of an earlier dense map ran out; its result is invalid");
+        return cbm::fail(CBM_B200_ERR_TIMEOUT, std::string(who) + ": a bounded wait of an earlier dense map or orthogonalised update ran out; its result is invalid");
     }
     return CBM_B200_OK;
 }

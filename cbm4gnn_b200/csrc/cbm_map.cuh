@@ -42,7 +42,7 @@ constexpr u64 WAIT_NS = 2000000000ULL;
 // Word that a kernel sets when one of its waits runs out; lives in page-locked host memory, so that
 // the next call can look at it without a synchronisation.  NULL on failure.
 int* timeout_word();
-// OK, or the error to return when an earlier map gave up waiting.
+// OK, or the error to return when an earlier kernel that has the word, a map or an update, gave up waiting.
 int check_timeout(const char* who);
 // SMs of the current device.
 int sm_count();
