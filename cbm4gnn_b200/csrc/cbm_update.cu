@@ -7,9 +7,11 @@
 // Precision: no entry of X, A or B exceeds 2.9, since none of their singular values does (X stays below 1.21).  So each is kept as
 // two fp16 terms of 2^12 times its value, h = fp16(v), l = fp16(v - h): 22 bits, down to 2^-37 of the largest, where fp16 ends.  A
 // product takes three fp16 MMAs, h h + h l + l h; l l is below 2^-22 of it.  (The dense maps, whose operands may have any
-// exponent, need three bf16 terms and six products.)  Against float64: 500 x 777 0.6 to 0.8e-6 of the result, where torch's fp32 products
-// give 2.4e-6.  As in cbm_map.cuh, an accumulator holds 64 columns of a contraction, the small products first, and is added to sums in
-// registers, because the tensor cores cut off towards zero at every step.
+// exponent, need three bf16 terms and six products, twice the time and a half more shared memory than there is for small matrices.)
+// Against float64: 500 x 777 0.6 to 0.8e-6 of the result, where torch's fp32 products give 2.4e-6.  That is of the whole: a row or
+// column far below the others meets the floor of 2^-37 sooner (see LOW), and a matrix that has one goes another way, plain_products.
+// As in cbm_map.cuh, an accumulator holds 64 columns of a contraction, the small products first, and is added to sums in registers,
+// because the tensor cores cut off towards zero at every step.
 //
 // Work: m (m + 1) n + m^2 (m + 1) + 2 m^2 n a step, as A and A A are symmetric: only tiles that reach the upper triangle are computed,
 // and the other half is written with them.
@@ -41,6 +43,8 @@ constexpr int THREADS = 256, PARTS = 64;  // of the norm
 constexpr int MAX_JOBS = 8;
 constexpr int PRODUCER = 8, ISSUER = 9, TILE_THREADS = 320;  // warps 0 - 7 add up and write
 constexpr int BOX_BYTES = 64 * 64 * 2;
+constexpr int SLICE = 128 * 128;                 // bytes: 128 rows of 64 columns of one term
+constexpr int SMALL_ARRAY = 4 * SLICE;           // [64 columns][term][row]
 
 struct Matrix {
     const float* g;  // update, or gradient
@@ -75,6 +79,7 @@ struct Matrix {
 struct Shape {
     __half *px[2], *pa, *pb;
     double* parts;             // [batch][PARTS]
+    int* low;                  // [batch]: whether it has stretches of rows or columns that two fp16 terms do not hold
     Matrix of;
     int m, n, ldx, lda, turned, batch;
     int tiles_sym, tiles_all;  // of one matrix: that reach the upper triangle of A, of X
@@ -92,6 +97,7 @@ struct Jobs {
     int nesterov;
     int* timeout;
     u32* arrived;              // of the products' blocks, zeroed by the first kernel
+    int* any_low;              // whether a matrix of the call has `low` set
 };
 
 enum Kind { GRAM, SQUARE, APPLY };
@@ -129,8 +135,25 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ J
     if (threadIdx.x == 0) {
         for (int i = 1; i < THREADS / 32; ++i) s += part[i];
         q.parts[b * PARTS + blockIdx.x] = s;
-        if (blockIdx.x == 0 && blockIdx.y == 0) *p.arrived = 0;
+        if (blockIdx.x == 0) q.low[b] = 0;
+        if (blockIdx.x == 0 && blockIdx.y == 0) *p.arrived = 0, *p.any_low = 0;
     }
+}
+
+// A matrix is low where a stretch of a row or column (32 values of larger matrices, up to 128 of small ones) that is not 0 has no value of LOW
+// of the norm.  In two fp16 terms rows of 128 x 512 whose largest value is 2^-16 of the norm come out with an error of 9e-7, at 2^-23 of 9e-5,
+// at 2^-30 of 9e-3, and below 2^-37 not at all; in fp32 all with 2e-7 (1 600 x 1 500: 5e-4 at 2^-26, 4e-7 in fp32).  The time of
+// fp32 is why it is not taken sooner: 2 048 x 4 096 13.1 ms, in two terms 1.12 (by a library's products 8.0); 64 x 500 369 us, 56 (439).
+constexpr float LOW = 1.f / (1 << 24);
+__device__ __forceinline__ u32 magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // (in the order of the values; NaN above all)
+__device__ __forceinline__ bool is_low(u32 most, float scale) { return most && most < __float_as_uint(LOW * scale); }
+
+__device__ __forceinline__ double norm_of(const Shape& q, int b) {  // (by a warp)
+    double s = 0.0;
+    for (int i = 0; i < PARTS; i += 32) s += __ldcg(&q.parts[b * PARTS + i + (threadIdx.x & 31)]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return sqrt(s);
 }
 
 __device__ __forceinline__ void split(float v, __half& h, __half& l) {
@@ -140,37 +163,56 @@ __device__ __forceinline__ void split(float v, __half& h, __half& l) {
 
 // X, split: 32 x 32 values to a block, through shared memory where it is turned.  Block x: a tile (of the largest job), y: a matrix.
 __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ Jobs p) {
+    constexpr int EACH = 32 * 32 / THREADS;
     __shared__ float turn[32][33];
+    __shared__ u32 s_column[32];
     cbm::wait_before();
     int j = 0, b = blockIdx.y;
     while (b >= p.job[j].batch) b -= p.job[j++].batch;
     const Shape& q = p.job[j];
     const int across = (q.n + 31) / 32, tiles = across * ((q.m + 31) / 32), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double s = 0.0;
-    for (int i = 0; i < PARTS; i += 32) s += q.parts[b * PARTS + i + lane];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const double scale = (double)SCALE / (sqrt(s) + (double)p.eps);
+    const double scale = (double)SCALE / (norm_of(q, b) + (double)p.eps);
+    bool low = false;
     const int64_t plane = (int64_t)q.m * q.ldx;
     __half* x = q.px[0] + 2 * b * plane;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int r0 = t / across * 32, c0 = t % across * 32;
-        if (q.turned) {
-            __syncthreads();
+        if (q.turned) {  // (the barrier at the end is behind the last tile's reads)
             for (int i = warp; i < 32; i += THREADS / 32)
                 if (c0 + i < q.n && r0 + lane < q.m) turn[i][lane] = update_at(p, q, b, c0 + i, r0 + lane);
             __syncthreads();
         }
-        for (int i = warp; i < 32; i += THREADS / 32)
+        float v[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int i = warp + e * (THREADS / 32);
+            v[e] = r0 + i < q.m && c0 + lane < q.n ? (q.turned ? turn[lane][i] : update_at(p, q, b, r0 + i, c0 + lane)) : 0.f;
+        }
+        u32 column = 0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int i = warp + e * (THREADS / 32);
+            v[e] = (float)((double)v[e] * scale);
+            column = max(column, magnitude(v[e]));
+            low |= is_low(__reduce_max_sync(0xffffffffu, magnitude(v[e])), SCALE);
             if (r0 + i < q.m && c0 + lane < q.n) {
-                const float u = q.turned ? turn[lane][i] : update_at(p, q, b, r0 + i, c0 + lane);
                 __half h, l;
-                split((float)((double)u * scale), h, l);
+                split(v[e], h, l);
                 const int64_t at = (int64_t)(r0 + i) * q.ldx + c0 + lane;
                 x[at] = h;
                 x[at + plane] = l;
             }
+        }
+        // a column is low where all that warps have of it is
+        if (__syncthreads_or(is_low(column, SCALE))) {
+            if (warp == 0) s_column[lane] = 0;
+            __syncthreads();
+            atomicMax(&s_column[lane], column);
+            __syncthreads();
+            if (warp == 0) low |= is_low(s_column[lane], SCALE);
+        }
     }
+    if (low) q.low[b] = 1, *p.any_low = 1;
 }
 
 // ---- products -------------------------------------------------------------------------------------
@@ -402,6 +444,166 @@ __device__ __forceinline__ void all_blocks(u32* arrived, u32 due, volatile int* 
     if (fetches) asm volatile("fence.proxy.async;" ::: "memory");
 }
 
+// ---- matrices with rows or columns far below the others ----------------------------------------------
+// The steps in fp32 without tensor cores, by `blocks` blocks that meet in `sync` between products, what they wrote then seen by all.  256
+// threads to a tile, of 128 x 128 beside pairs of blocks, else 64 x 64: 64 products to 16 values out of shared memory, or 16 to 8; the next piece of the contraction is on its way meanwhile.  X, A and B lie where their two terms would.  Of A and
+// B half the tiles are computed: the other half comes out the same, as its products commute.
+constexpr int PLAIN_VALUES = 2048, PLAIN_SMEM = 4 * 32 * (64 + 4) * 4;  // of an operand's piece; bytes for two pieces of both
+static_assert(PLAIN_SMEM >= 4 * 16 * (128 + 4) * 4 && PLAIN_SMEM <= SMALL_ARRAY && PLAIN_SMEM <= Sizes<SINGLE>::STAGES * Sizes<SINGLE>::STAGE,
+              "operands lie where the tensor cores' would");
+
+// sum = rows from i0 on of `first` times rows (or, ACROSS, columns) from j0 on of `second`, whose rows start at multiples of 16 bytes.
+template <int TILE, bool ACROSS>
+__device__ __forceinline__ void plain_tile(const float* first, int ld1, int rows1, int i0, const float* second, int ld2, int width, int j0, int deep,
+                                           float* smem, float (&sum)[TILE / 16][TILE / 16]) {
+    constexpr int DEEP = PLAIN_VALUES / TILE, PITCH = TILE + 4, PIECE = DEEP * PITCH, EACH = TILE / 16;
+    const int at = threadIdx.x, ty = at >> 4, tx = at & 15;
+    const bool works = at < 256;
+    float4 a[2], b[2];
+    auto row_of = [&](const float* from, int ld, int rows, int r, int k) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && k < deep) {
+            v = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)r * ld + k));
+            if (k + 1 >= deep) v.y = 0.f;
+            if (k + 2 >= deep) v.z = 0.f;
+            if (k + 3 >= deep) v.w = 0.f;
+        }
+        return v;
+    };
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = at + 256 * e, r = i / (DEEP / 4), k = k0 + 4 * (i % (DEEP / 4));
+            a[e] = row_of(first, ld1, rows1, i0 + r, k);
+            if constexpr (ACROSS) {  // (columns past the last make results past the last)
+                const int d = k0 + i / (TILE / 4), j = j0 + 4 * (i % (TILE / 4));
+                b[e] = d < deep && j < width ? __ldcg(reinterpret_cast<const float4*>(second + (int64_t)d * ld2 + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+                b[e] = row_of(second, ld2, width, j0 + r, k);
+            }
+        }
+    };
+    auto put = [&](float* to) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int i = at + 256 * e, r = i / (DEEP / 4), k = 4 * (i % (DEEP / 4));
+            to[k * PITCH + r] = a[e].x, to[(k + 1) * PITCH + r] = a[e].y, to[(k + 2) * PITCH + r] = a[e].z, to[(k + 3) * PITCH + r] = a[e].w;
+            float* const next = to + PIECE;
+            if constexpr (ACROSS) *reinterpret_cast<float4*>(next + i / (TILE / 4) * PITCH + 4 * (i % (TILE / 4))) = b[e];
+            else next[k * PITCH + r] = b[e].x, next[(k + 1) * PITCH + r] = b[e].y, next[(k + 2) * PITCH + r] = b[e].z, next[(k + 3) * PITCH + r] = b[e].w;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) sum[i][j] = 0.f;
+    __syncthreads();  // (the last tile's reads)
+    if (works) fetch(0), put(smem);
+    int turn = 0;
+    for (int k0 = 0; k0 < deep; k0 += DEEP, turn ^= 1) {
+        __syncthreads();
+        if (!works) continue;
+        const bool more = k0 + DEEP < deep;
+        if (more) fetch(k0 + DEEP);
+        const float* const from = smem + turn * 2 * PIECE;
+#pragma unroll 4
+        for (int k = 0; k < DEEP; ++k) {
+            float u[EACH], v[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; i += 4) {
+                *reinterpret_cast<float4*>(&u[i]) = *reinterpret_cast<const float4*>(from + k * PITCH + 16 * i + 4 * ty);
+                *reinterpret_cast<float4*>(&v[i]) = *reinterpret_cast<const float4*>(from + PIECE + k * PITCH + 16 * i + 4 * tx);
+            }
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+#pragma unroll
+                for (int j = 0; j < EACH; ++j) sum[i][j] += u[i] * v[j];
+        }
+        if (more) put(smem + (turn ^ 1) * 2 * PIECE);
+    }
+}
+
+struct Plain {
+    float *x[2], *gram, *poly;
+    __device__ __forceinline__ Plain(const Shape& q, int b) {
+        x[0] = reinterpret_cast<float*>(q.px[0]) + (int64_t)b * q.m * q.ldx, x[1] = reinterpret_cast<float*>(q.px[1]) + (int64_t)b * q.m * q.ldx;
+        gram = reinterpret_cast<float*>(q.pa) + (int64_t)b * q.m * q.lda, poly = reinterpret_cast<float*>(q.pb) + (int64_t)b * q.m * q.lda;
+    }
+};
+// Tiles first, first + blocks, ... of a product of a matrix, of `tiles`, `across` in a row.
+template <int TILE, bool ACROSS>
+__device__ __forceinline__ void plain_product(const Shape& q, int b, Kind kind, int from, bool last, int first, int blocks, float* smem) {
+    const Plain is(q, b);
+    const int m = q.m, width = kind == APPLY ? q.n : m, across = (width + TILE - 1) / TILE, down = (m + TILE - 1) / TILE;
+    const int tiles = kind == APPLY ? across * down : across * (across + 1) / 2;
+    for (int t = first; t < tiles; t += blocks) {
+        int i0 = t / across, j0 = t % across;
+        if (kind != APPLY) {
+            i0 = 0, j0 = t;
+            for (int left = across; j0 >= left; left = across - i0) j0 -= left, ++i0;
+            j0 += i0;
+        }
+        i0 *= TILE, j0 *= TILE;
+        float sum[TILE / 16][TILE / 16];
+        if (kind == GRAM) plain_tile<TILE, ACROSS>(is.x[from], q.ldx, m, i0, is.x[from], q.ldx, m, j0, q.n, smem, sum);
+        else plain_tile<TILE, ACROSS>(kind == SQUARE ? is.gram : is.poly, q.lda, m, i0, ACROSS ? is.x[from] : is.gram, ACROSS ? q.ldx : q.lda, width, j0, m, smem, sum);
+        if (threadIdx.x >= 256) continue;
+#pragma unroll
+        for (int i = 0; i < TILE / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < TILE / 16; ++j) {
+                const int r = i0 + i / 4 * 64 + 4 * (threadIdx.x >> 4) + i % 4, c = j0 + j / 4 * 64 + 4 * (threadIdx.x & 15) + j % 4;
+                if (r >= m || c >= width) continue;
+                float v = sum[i][j];
+                if constexpr (!ACROSS) {
+                    if (kind == SQUARE) v = QUINTIC_C * v + QUINTIC_B * __ldcg(is.gram + (int64_t)r * q.lda + c);
+                    float* const to = kind == GRAM ? is.gram : is.poly;
+                    to[(int64_t)r * q.lda + c] = v;
+                    if (j0 != i0) to[(int64_t)c * q.lda + r] = v;
+                } else {
+                    v += QUINTIC_A * __ldcg(is.x[from] + (int64_t)r * q.ldx + c);
+                    const float o[8] = {SCALE * v};
+                    if (!last) is.x[from ^ 1][(int64_t)r * q.ldx + c] = v;
+                    else if (q.turned) q.of.write(b, c, r, 1, o);
+                    else q.of.write(b, r, c, 1, o);
+                }
+            }
+    }
+}
+
+// Matrix `only` of the first job, whose norm is given, or all that have `low` set.
+template <int TILE, class Sync>
+__device__ __noinline__ void plain_products(const Jobs& p, const Shape* jobs, int only, double norm, int steps, int rank, int blocks, float* smem, Sync sync) {
+    auto each = [&](auto&& f) {
+        if (only >= 0) return f(jobs[0], only);
+        for (int j = 0; j < p.count; ++j)
+            for (int b0 = 0; b0 < jobs[j].batch; b0 += 32) {
+                const int b = b0 + (threadIdx.x & 31);
+                for (u32 set = __ballot_sync(0xffffffffu, b < jobs[j].batch && __ldcg(&jobs[j].low[b])); set; set &= set - 1) f(jobs[j], b0 + __ffs(set) - 1);
+            }
+    };
+    each([&](const Shape& q, int b) {
+        float* const x = Plain(q, b).x[0];
+        const double scale = 1.0 / ((only >= 0 ? norm : norm_of(q, b)) + (double)p.eps);
+        for (int i = rank; i < q.m; i += blocks)
+            for (int j = threadIdx.x; j < q.n; j += blockDim.x)
+                x[(int64_t)i * q.ldx + j] = (float)((double)(q.turned ? update_at(p, q, b, j, i) : update_at(p, q, b, i, j)) * scale);
+    });
+    sync();
+    for (int k = 0; k < steps; ++k)
+        for (int kind = GRAM; kind <= APPLY; ++kind) {
+            int at = rank;  // this block's next tile, from where a matrix' tiles begin
+            each([&](const Shape& q, int b) {
+                const int width = kind == APPLY ? q.n : q.m;
+                const int across = (width + TILE - 1) / TILE, tiles = kind == APPLY ? across * ((q.m + TILE - 1) / TILE) : across * (across + 1) / 2;
+                if (kind == APPLY) plain_product<TILE, true>(q, b, APPLY, k & 1, k + 1 == steps, at, blocks, smem);
+                else plain_product<TILE, false>(q, b, (Kind)kind, k & 1, false, at, blocks, smem);
+                at = ((at - tiles) % blocks + blocks) % blocks;
+            });
+            sync();
+        }
+}
+
 // All products of all matrices, one kind after the other: as launches of their own each of the fifteen took 5 to 8 us before its first MMA.
 template <Mode MODE>
 __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const int sym_tiles, const int all_tiles,
@@ -412,7 +614,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
     extern __shared__ unsigned char smem_raw[];
     __shared__ u64 s_bar[2 * S::STAGES + 2 * S::ACCS + 1];
     __shared__ u32 s_tmem;
-    __shared__ int s_gave_up;
+    __shared__ int s_gave_up, s_any_low;
     // (at an index that is not known beforehand, parameters are read from the constant bank at hundreds of cycles a time)
     __shared__ Shape s_jobs[MAX_JOBS];
     const u32 smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -531,6 +733,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         float4* turn = reinterpret_cast<float4*>(smem_raw + (smem - smem_u32(smem_raw)) + S::STAGES * S::STAGE) + warp * (S::TURN / 16);
         u32 it = 0;
         bool ok = true;
+        const bool any_low = __any_sync(0xffffffffu, __ldcg(p.any_low) != 0);
+        if (threadIdx.x == 0) s_any_low = any_low;
         each_product([&](Kind kind, int from, bool last) {
           for (int t = rank; t < tiles_of(kind) && ok; t += stride) {
             const Where w = tile_of<S::ROWS, BN>(s_jobs, kind, t);
@@ -639,7 +843,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
                             if (r < m && c + 8 * i < width) t.store(out, plane);
                         }
                     }
-                } else {
+                } else if (!any_low || !__any_sync(0xffffffffu, __ldcg(&q.low[w.matrix]))) {  // (of the others the result comes at the end)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float v[8];
@@ -673,6 +877,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
         if constexpr (TWO) pair_free(tmem);
         else tmem_free(tmem);
     }
+    // Matrices that have to go another way, once nobody reads what lies in their place.  (Here, and not ahead of the others: a question about each
+    // tile in the loops above costs all matrices 4 %.)
+    if (!s_any_low) return;
+    u32 due = (3 * steps - 1) * gridDim.x;
+    const auto sync = [&] { all_blocks(p.arrived, due += gridDim.x, gave_up, p.timeout, false, false); };
+    sync();
+    plain_products<TWO ? 128 : 64>(p, s_jobs, -1, 0.0, steps, blockIdx.x, gridDim.x, reinterpret_cast<float*>(smem_raw + (smem - smem_u32(smem_raw))), sync);
 }
 
 // ---- small matrices -------------------------------------------------------------------------------
@@ -682,8 +893,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_c
 // cluster's shared memory, each block joining some rows for all; A A is computed by every block for itself, and B X is a matter of its
 // own columns.  X serves both products as it lies: its rows are the contraction of one and the columns of the other.
 constexpr int SMALL_THREADS = 512, SMALL_COLS = 128, SMALL_BLOCKS = 8;
-constexpr int SLICE = 128 * 128;                 // bytes: 128 rows of 64 columns of one term
-constexpr int SMALL_ARRAY = 4 * SLICE;           // [64 columns][term][row]
 constexpr int SMALL_SMEM = 3 * SMALL_ARRAY + 1024;
 
 __device__ __forceinline__ void cluster_barrier_async() {
@@ -727,6 +936,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     __shared__ u32 s_tmem;
     __shared__ int s_gave_up;
     __shared__ double s_part[SMALL_THREADS / 32], s_norm[SMALL_BLOCKS];
+    __shared__ double s_low;  // the norm of a matrix that has low rows or columns, -1: it has none
+    __shared__ u32 s_across[128], s_least, s_lows[SMALL_BLOCKS];  // largest across rows of the update; least of the largest that are not 0
     const u32 smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     unsigned char* const base = smem_raw + (smem - smem_u32(smem_raw));
     unsigned char *const xs = base, *const as = base + SMALL_ARRAY, *const bs = base + 2 * SMALL_ARRAY;
@@ -738,8 +949,11 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     if (threadIdx.x == 0) {
         bar_init(bar, 1);
         s_gave_up = 0;
+        s_least = 0xffffffffu;
+        s_low = -1.0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x < 128) s_across[threadIdx.x] = 0;
     fence_before();
     cluster_barrier();
     fence_after();
@@ -756,6 +970,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     const bool turned = q.turned;
     cbm::wait_before();
 
+    int by_terms = steps;
     // ---- momentum, norm, X
     auto at_sum = [&](int r, int c) -> float& { return sums[r * 128 + (((c >> 2) ^ (r & 31)) << 2) + (c & 3)]; };
     {
@@ -764,6 +979,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         const float* const g = of.g + b * of.next_g + (turned ? c0 * of.ldg : c0);
         float* const mom = of.m ? of.m + (turned ? c0 * of.ldm : c0) : nullptr;
         constexpr int AT_ONCE = 2;  // rows, of four values a lane each, which are fetched together
+        u32 least = 0xffffffffu, across[4] = {0, 0, 0, 0};
 #pragma unroll 1
         for (int i0 = warp; i0 < slow; i0 += AT_ONCE * (SMALL_THREADS / 32)) {
             float u[AT_ONCE][4], mm[AT_ONCE][4];
@@ -777,7 +993,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
                     mm[h][e] = fetch1(mom + (on ? i * of.ldm + j : 0), on && mom);
                 }
 #pragma unroll
-            for (int h = 0; h < AT_ONCE; ++h)
+            for (int h = 0; h < AT_ONCE; ++h) {
+                u32 most = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = i0 + h * (SMALL_THREADS / 32), j = lane + 32 * e;
@@ -789,20 +1006,39 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
                     }
                     at_sum(turned ? j : i, turned ? i : j) = u[h][e];
                     s += (double)u[h][e] * u[h][e];
+                    most = max(most, magnitude(u[h][e])), across[e] = max(across[e], magnitude(u[h][e]));
                 }
+                most = __reduce_max_sync(0xffffffffu, most);
+                if (most) least = min(least, most);
+            }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) s_part[warp] = s;
+        if (lane == 0) s_part[warp] = s, atomicMin(&s_least, least);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) atomicMax(&s_across[lane + 32 * e], across[e]);
         __syncthreads();
+        if (warp == 0) {
+            least = s_least;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (const u32 most = s_across[lane + 32 * e]) least = min(least, most);
+            least = __reduce_min_sync(0xffffffffu, least);
+        }
         if (threadIdx.x < blocks) {
             s = 0.0;
             for (int i = 0; i < SMALL_THREADS / 32; ++i) s += s_part[i];
             asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_block(smem_u32(&s_norm[rank]), threadIdx.x)), "d"(s) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(smem_u32(&s_lows[rank]), threadIdx.x)), "r"(least) : "memory");
         }
         cluster_barrier();
         s = 0.0;
-        for (int i = 0; i < blocks; ++i) s += s_norm[i];
+        least = 0xffffffffu;
+        for (int i = 0; i < blocks; ++i) s += s_norm[i], least = min(least, s_lows[i]);
+        if (least < __float_as_uint(INFINITY) && (double)__uint_as_float(least) < (double)LOW * (sqrt(s) + (double)p.eps)) {
+            if (threadIdx.x == 0) s_low = sqrt(s);
+            by_terms = 0;  // (see the end)
+        }
         const Scale scale((double)SCALE / (sqrt(s) + (double)p.eps));
 #pragma unroll 1
         for (int i = threadIdx.x; i < 128 * 16; i += SMALL_THREADS) {  // eight values: row i / 16, columns from 8 (i % 16) on
@@ -863,7 +1099,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     const u32 both = idesc_half(128, 256, false), one = idesc_half(128, 128, false);
     const int deep = (m + 63) / 64, wide = (cols + 63) / 64;  // slices of 64 of a contraction over rows, of this block's columns
 #pragma unroll 1
-    for (int k = 0; k < steps; ++k) {
+    for (int k = 0; k < by_terms; ++k) {
         // ---- A = X X^T
         if (active > rank) {
             if (warp == 0)
@@ -1012,6 +1248,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     __syncthreads();
     fence_after();
     if (warp == 0) tmem_free(tmem);
+    if (s_low >= 0.0)
+        plain_products<64>(p, &q, b, s_low, steps, rank, blocks, reinterpret_cast<float*>(xs), [] { cluster_barrier(); });
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -1047,14 +1285,16 @@ int64_t pad(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t lay_out(Shape* q, int rows, int cols, int batch, unsigned char* at) {
     const int m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
     const int ldx = (n + 7) / 8 * 8, lda = (m + 7) / 8 * 8;
-    const int64_t x = pad((int64_t)4 * batch * m * ldx), a = pad((int64_t)4 * batch * m * lda), parts = pad((int64_t)8 * batch * PARTS);
+    const int64_t x = pad((int64_t)4 * batch * m * ldx), a = pad((int64_t)4 * batch * m * lda), parts = pad((int64_t)8 * batch * PARTS),
+                  low = pad((int64_t)4 * batch);
     if (q) {
         q->m = m, q->n = n, q->ldx = ldx, q->lda = lda, q->turned = rows > cols, q->batch = batch;
         q->px[0] = reinterpret_cast<__half*>(at), q->px[1] = reinterpret_cast<__half*>(at + x);
         q->pa = reinterpret_cast<__half*>(at + 2 * x), q->pb = reinterpret_cast<__half*>(at + 2 * x + a);
         q->parts = reinterpret_cast<double*>(at + 2 * x + 2 * a);
+        q->low = reinterpret_cast<int*>(at + 2 * x + 2 * a + parts);
     }
-    return 2 * x + 2 * a + parts;
+    return 2 * x + 2 * a + parts + low;
 }
 
 template <Mode MODE>
@@ -1155,7 +1395,7 @@ int run(const char* who, Jobs& p, bool small, int steps, void* stream) {
     return e == cudaSuccess ? CBM_B200_OK : cbm::fail(CBM_B200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
-constexpr int HEAD = 256;  // of a workspace: the count of blocks
+constexpr int HEAD = 256;  // of a workspace: the count of blocks, and whether a matrix has low rows or columns
 constexpr int MAX_SIDE = 1 << 16, MAX_BATCH = 32768;  // (tiles are counted in 31 bits, matrices in a grid's second dimension)
 
 }  // namespace
@@ -1175,7 +1415,7 @@ extern "C" int cbm_b200_orthogonalise(const float* u, int64_t ldu, int64_t next_
     if (workspace_bytes < cbm_b200_orthogonalise_workspace(batch, rows, cols)) return cbm::fail(CBM_B200_ERR_ARG, "orthogonalise: workspace too small");
     Jobs p{};
     p.count = 1, p.eps = eps;
-    p.arrived = static_cast<u32*>(workspace);
+    p.arrived = static_cast<u32*>(workspace), p.any_low = static_cast<int*>(workspace) + 1;
     lay_out(&p.job[0], rows, cols, batch, static_cast<unsigned char*>(workspace) + HEAD);
     p.job[0].of = Matrix{u, nullptr, nullptr, out, ldu, 0, 0, ldout, next_u, next_out, 0.f, 0.f};
     return run("orthogonalise", p, is_small(p.job[0].m, p.job[0].n), steps, stream);
@@ -1210,6 +1450,7 @@ extern "C" int cbm_b200_orthogonal_step(const cbm_b200_update_of* of, int32_t co
     for (int i = 0; i < count;) {
         Jobs p{};
         p.eps = eps, p.momentum = momentum, p.nesterov = nesterov, p.arrived = static_cast<u32*>(workspace);
+        p.any_low = static_cast<int*>(workspace) + 1;
         for (; i < count && p.count < MAX_JOBS; ++i) {
             const cbm_b200_update_of& u = of[i];
             if (u.rows == 0 || u.cols == 0) continue;

@@ -204,3 +204,90 @@ def test_sizes_past_the_limits_are_refused_by_name():
     tall = _normal(1, 65_536, 2)
     want, bound = ortho64(tall, 5)
     assert (orthogonalise(tall).double() - want).norm() <= bound
+
+
+def _low_update(seed, m, n, by_rows, powers):
+    """A random update of which an eighth of the rows (or columns) lies lower, for each of the powers."""
+    u = _normal(seed, m, n)
+    side = m if by_rows else n
+    scale = torch.ones(side, device="cuda")
+    for k, power in enumerate(powers):
+        scale[k * side // 8:(k + 1) * side // 8] = power
+    return u * (scale[:, None] if by_rows else scale[None, :])
+
+
+def _stretch_bound(u, by_rows, floor):
+    """The result in 64 bits, and how far each row (or column) of it may be off.
+
+    A step: what is there grows by at most a.  New: values stored, products without their smallest part, and their sums, each some 2^-22
+    of a row of |X| or |B| times |X|, whose norm is at most that of the row times the root of the shorter side (16 of them); and where
+    two fp16 terms hold the operands the floor of 2^-37 under a row's entries, and under those of A (b and 2 c times, times X,
+    whose norm is 1.21) and B."""
+    m, n = u.shape
+    turned = m > n
+    x = u.double()
+    x = x / (x.norm() + 1e-7)
+    x = x.t() if turned else x
+    along = 1 if by_rows != turned else 0   # rows, or columns, of x
+    a, b, c = 3.4445, -4.7750, 2.0315
+    short, length = min(m, n), x.size(along)
+    off = torch.zeros(x.size(1 - along), dtype=torch.float64, device="cuda")
+    for _ in range(5):
+        g = x @ x.t()
+        x = a * x + (b * g + c * g @ g) @ x
+        off = a * off + 16 * 2.0 ** -22 * short ** 0.5 * x.norm(dim=along)
+        if floor:
+            off = off + 2.0 ** -37 * (2 * length ** 0.5 + (12 * short ** 0.5 if along == 1 else 0.0))
+    return (x.t() if turned else x), off
+
+
+@pytest.mark.parametrize("m,n", [(128, 512), (100, 900), (30, 20), (300, 700), (500, 400), (1600, 1500), (65, 1100), (129, 129)])
+@pytest.mark.parametrize("by_rows", [True, False])
+@pytest.mark.parametrize("powers", [(1e-3,), (1e-4, 1e-5), (1e-7,), (1e-5, 1e-9, 1e-20), (0.0, 1e-12)])
+def test_low_rows_and_columns_of_an_update_keep_their_digits(m, n, by_rows, powers):
+    """Whatever lies beside them: down to 2^-24 of the norm in two fp16 terms, whose floor is 2^-37 of it, below that in fp32."""
+    u = _low_update(m + n, m, n, by_rows, powers)
+    along = 1 if by_rows else 0
+    got = orthogonalise(u).double()
+    want, off = _stretch_bound(u, by_rows, floor=min(p for p in powers if p) > 1e-6)
+    wrong = (got - want).norm(dim=along)
+    assert (wrong <= off).all(), (wrong / off).max()
+
+
+def test_low_blocks_stacks_lists_and_replays():
+    """Matrices that go by fp32 products beside others that do not."""
+    stack = torch.stack([_low_update(i, 200, 330, True, (1e-9,) if i in (1, 4) else ()) for i in range(5)])
+    got = orthogonalise(stack)
+    for i in range(5):
+        want, off = _stretch_bound(stack[i], True, floor=False)
+        assert ((got[i].double() - want).norm(dim=1) <= off + (0 if i in (1, 4) else 2.0 ** -30)).all()
+        assert torch.equal(got[i], orthogonalise(stack[i]))
+    small = torch.stack([_low_update(i, 90, 60, False, (1e-9,) if i == 2 else ()) for i in range(4)])
+    for i, o in enumerate(orthogonalise(small)):
+        assert torch.equal(o, orthogonalise(small[i]))
+    tiny = _normal(9, 40, 300) * 1e-13     # all of it far below eps
+    for u in (tiny, _normal(8, 400, 300) * 1e-13):
+        want, off = _stretch_bound(u, True, floor=False)
+        assert ((orthogonalise(u).double() - want).norm(dim=1) <= off).all()
+    shapes = [(64, 100), (300, 200), (128, 128), (16, 600), (500, 64), (90, 1000)]
+    for chosen in (shapes, [s for s in shapes if min(s) <= 128 and max(s) <= 1024]):   # tiles beside one another, clusters
+        ws = [_normal(i, *s) for i, s in enumerate(chosen)]
+        gs = [_low_update(10 + i, *s, i % 2 == 0, (1e-10, 1e-6) if i % 3 else ()) for i, s in enumerate(chosen)]
+        ms = [_low_update(30 + i, *s, i % 2 == 0, (1e-10, 1e-6) if i % 3 else ()) for i, s in enumerate(chosen)]
+        start = [t.clone() for t in ws + ms]
+        graph = torch.cuda.CUDAGraph()
+        step = lambda: orthogonal_step(ws, gs, ms, lr=0.05, momentum=0.9)  # noqa: E731, B023
+        step()
+        after = [t.clone() for t in ws + ms]
+        for w, w0, g, m0 in zip(ws, start, gs, start[len(ws):]):
+            m1 = 0.9 * m0.double() + g.double()
+            o, bound = ortho64(g.double() + 0.9 * m1, 5)
+            f = 0.05 * max(1.0, w.size(0) / w.size(1)) ** 0.5
+            assert (w.double() - (w0.double() - f * o)).norm() <= f * (bound + 2e-4 * 2.0 ** -3) + 2.0 ** -23 * w0.double().norm()
+        with torch.cuda.graph(graph):
+            step()
+        for to, of in zip(ws + ms, start):
+            to.copy_(of)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(after, ws + ms))
