@@ -10,7 +10,7 @@
 //   * Samples of up to a tile's rows: a team of threads reads a sample, joins its sums in registers or shared memory and reads it again,
 //     out of L1 or L2, to write the results.  Tiles end where samples do, so that each of these is one team's.
 //   * Longer samples: every tile leaves a partial result, a warp or a block to a sample joins them in a fixed order, and a third kernel
-//     goes over the rows again, from their ends, which L2 still holds.
+//     goes over the rows again, from their ends, of which L2 still holds some (of 307 MB 41, in the gradient 47 of 614).
 //   * A few samples of some hundred rows: a cluster of blocks to each, which join through one another's shared memory: one launch.
 //   * Groups wider than a block's threads hold: a block to each, value by value, with sums in 64 bits.
 // Elsewhere means and squares around them are kept for every few rows and joined (mean and sum of squares around it of two parts give those
@@ -54,6 +54,9 @@ __device__ __forceinline__ float param(const void* w, int wide, int c, float non
     return !w ? none : wide ? static_cast<const float*>(w)[c] : cbm::widen(static_cast<const T*>(w)[c]);
 }
 
+// By the fast forms: exp's argument and the quotient's are rounded once more, |z| U and 2 U of the result, where z itself comes with a
+// rounding of |z| U.  (With expf and a division 1 000 000 x 64 bf16 in samples of 2 300 rows 143 us instead of 127, with the gradient 352
+// instead of 270; 262 147 x 100 bf16 in samples of 30 84 and 67, 256 and 172.)
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 template <int ACT>
 __device__ __forceinline__ float activated(float z) {
@@ -143,6 +146,8 @@ __device__ __forceinline__ float2 group_sum(float2 v, const RowShape& h, float2 
     return v;
 }
 
+// (Bounded to the 64 registers that 1 024 threads may have, as the widest groups need; the gradient of eight values spills 316 to 420 bytes a
+// thread for that, also where groups have 256 threads.)
 template <class T, int E, bool STRIDED, bool GRAD>
 __global__ void __launch_bounds__(1024) rows_kernel(const Params p, const RowShape h) {
     __shared__ float2 s_warp[2][32];
@@ -380,7 +385,7 @@ struct All {
 };
 // The gradient's vectors of 16 bytes come through shared memory, where each thread has DEPTH places of its own: rows ahead take no registers,
 // the code of a turn is that of one row, and the rows of a short sample are still there when they are asked for again.  (1 000 000 x 64 bf16 in
-// samples of 2 300 rows, with the gradient 465 -> 364 us; 235 868 x 256 fp32 350 -> 346.  Narrower vectors lose: 262 147 x 100 bf16 by pairs
+// samples of 2 300 rows, with the gradient 465 -> 364 us; 235 868 x 256 fp32 350 -> 342.  Narrower vectors lose: 262 147 x 100 bf16 by pairs
 // 262 -> 290; so does the forward pass, whose turns are short: 102 -> 143.)
 template <class T, int E, bool STRIDED, bool GRAD>
 struct Ring {
@@ -510,7 +515,9 @@ __device__ __forceinline__ void fetch_params(const Params& p, const Team& t, flo
     }
 }
 
-// Blocks of an SM: with one more their registers spill to a few hundred bytes a thread, with one fewer too little is on its way.
+// Blocks of an SM: with one fewer too little is on its way.  Some forms spill registers at that, by -Xptxas -v: tiles of single values up to
+// 460 bytes a thread, of pairs in the gradient 224, of four fp32 144, of eight 16-bit ones 144; clusters of single values up to 916.  With
+// one block more all of them do.
 constexpr int blocks_resident(int e, bool grad) { return e == 8 ? (grad ? 2 : 3) : e == 4 && grad ? 3 : 4; }
 
 // What a thread finds in `rows` rows of a sample from row lo on: the mean over its values and the squares around it; or, for the gradient,
@@ -1097,7 +1104,9 @@ struct Plan {
         way = TILES;
         slab_groups = THREADS / lanes < GROUPS ? THREADS / lanes : GROUPS;
         if (groups < slab_groups) slab_groups = groups;
-        // A few samples whose rows a cluster goes over in some dozen turns: 1 000 x 64 fp32 12 us, 15 with tiles, joins and rows by themselves.
+        // A few samples whose rows a cluster goes over in some dozen turns, with tiles, joins and rows by themselves above (x 64 fp32, turns of
+        // 128 rows, out of DRAM): one of 1 000 rows 10 us, by tiles 16, with the gradient 21 and 29; one of 3 000 14 and 18, 33 both; 16 of 6 000 26
+        // and 41, 62 and 72, but one of 6 000 20 and 18, 49 and 33; past the limit 16 of 12 000 47 and 51, 117 and 102, one 33 and 23, 82 and 39.
         const int64_t slabs = (groups + slab_groups - 1) / slab_groups, turn = (int64_t)CLUSTER * (THREADS / (slab_groups * lanes));
         if (!ptr && rows_each > 1 && n_samples * CLUSTER * slabs <= 2 * SMS && rows_each <= 48 * turn) {
             way = CLUSTERS;
@@ -1105,7 +1114,8 @@ struct Plan {
             parts = n_samples * CLUSTER;
             return;
         }
-        // Four rows at once, or where samples are short one, so that more of them are under way (262 147 x 100 bf16 in samples of 30 rows).
+        // Four rows at once, or where samples are short one, so that more of them are under way (262 147 x 100 bf16 with SiLU, samples of 30 rows:
+        // one at once 66 us, four 129; of 60 61 and 94; of 100 71 and 78, with the gradient 197 and 180; of 200 78 and 62, 184 and 150).
         const int wanted = (n_samples && n_rows / n_samples > 64 ? 4 : 1) * slab_groups * lanes;
         for (team = 32; team < THREADS && team < wanted;) team *= 2;
         const int at_once = team / (slab_groups * lanes);
