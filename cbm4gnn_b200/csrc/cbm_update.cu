@@ -140,11 +140,12 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ J
     }
 }
 
-// A matrix is low where a stretch of a row or column (32 values of larger matrices, up to 128 of small ones) that is not 0 has no value of LOW
-// of the norm.  In two fp16 terms rows of 128 x 512 whose largest value is 2^-16 of the norm come out with an error of 9e-7, at 2^-23 of 9e-5,
+// A matrix is low where a stretch of a row or column (32 values of larger matrices, up to 128 of small ones) with FEWEST or more that are not 0
+// has none of LOW of the norm.  (One value or two may be that small by chance.)  In two fp16 terms rows of 128 x 512 whose largest value is 2^-16 of the norm come out with an error of 9e-7, at 2^-23 of 9e-5,
 // at 2^-30 of 9e-3, and below 2^-37 not at all; in fp32 all with 2e-7 (1 600 x 1 500: 5e-4 at 2^-26, 4e-7 in fp32).  The time of
 // fp32 is why it is not taken sooner: 2 048 x 4 096 13.1 ms, in two terms 1.12 (by a library's products 8.0); 64 x 500 369 us, 56 (439).
 constexpr float LOW = 1.f / (1 << 24);
+constexpr int FEWEST = 4;
 __device__ __forceinline__ u32 magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // (in the order of the values; NaN above all)
 __device__ __forceinline__ bool is_low(u32 most, float scale) { return most && most < __float_as_uint(LOW * scale); }
 
@@ -165,7 +166,7 @@ __device__ __forceinline__ void split(float v, __half& h, __half& l) {
 __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ Jobs p) {
     constexpr int EACH = 32 * 32 / THREADS;
     __shared__ float turn[32][33];
-    __shared__ u32 s_column[32];
+    __shared__ u32 s_column[32], s_values[32];
     cbm::wait_before();
     int j = 0, b = blockIdx.y;
     while (b >= p.job[j].batch) b -= p.job[j++].batch;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ 
             const int i = warp + e * (THREADS / 32);
             v[e] = (float)((double)v[e] * scale);
             column = max(column, magnitude(v[e]));
-            low |= is_low(__reduce_max_sync(0xffffffffu, magnitude(v[e])), SCALE);
+            if (is_low(__reduce_max_sync(0xffffffffu, magnitude(v[e])), SCALE)) low |= __popc(__ballot_sync(0xffffffffu, magnitude(v[e]))) >= FEWEST;
             if (r0 + i < q.m && c0 + lane < q.n) {
                 __half h, l;
                 split(v[e], h, l);
@@ -205,11 +206,15 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const __grid_constant__ 
         }
         // a column is low where all that warps have of it is
         if (__syncthreads_or(is_low(column, SCALE))) {
-            if (warp == 0) s_column[lane] = 0;
+            if (warp == 0) s_column[lane] = s_values[lane] = 0;
             __syncthreads();
+            u32 values = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) values += magnitude(v[e]) != 0;
             atomicMax(&s_column[lane], column);
+            atomicAdd(&s_values[lane], values);
             __syncthreads();
-            if (warp == 0) low |= is_low(s_column[lane], SCALE);
+            if (warp == 0) low |= s_values[lane] >= FEWEST && is_low(s_column[lane], SCALE);
         }
     }
     if (low) q.low[b] = 1, *p.any_low = 1;
@@ -605,6 +610,7 @@ __device__ __noinline__ void plain_products(const Jobs& p, const Shape* jobs, in
 }
 
 // All products of all matrices, one kind after the other: as launches of their own each of the fifteen took 5 to 8 us before its first MMA.
+// (320 threads may have 168 registers each; pairs, whose warps add up 64 columns, spill some 204 bytes of them a thread, single blocks none.)
 template <Mode MODE>
 __global__ void __launch_bounds__(TILE_THREADS, 1) product_kernel(const __grid_constant__ Jobs p, const int sym_tiles, const int all_tiles,
                                                                   const int steps) {
@@ -937,7 +943,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     __shared__ int s_gave_up;
     __shared__ double s_part[SMALL_THREADS / 32], s_norm[SMALL_BLOCKS];
     __shared__ double s_low;  // the norm of a matrix that has low rows or columns, -1: it has none
-    __shared__ u32 s_across[128], s_least, s_lows[SMALL_BLOCKS];  // largest across rows of the update; least of the largest that are not 0
+    // largest across rows of the update, and how many are not 0; least of the largest of those with enough
+    __shared__ u32 s_across[128], s_values[128], s_least, s_lows[SMALL_BLOCKS];
     const u32 smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     unsigned char* const base = smem_raw + (smem - smem_u32(smem_raw));
     unsigned char *const xs = base, *const as = base + SMALL_ARRAY, *const bs = base + 2 * SMALL_ARRAY;
@@ -953,7 +960,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         s_low = -1.0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (threadIdx.x < 128) s_across[threadIdx.x] = 0;
+    if (threadIdx.x < 128) s_across[threadIdx.x] = s_values[threadIdx.x] = 0;
     fence_before();
     cluster_barrier();
     fence_after();
@@ -979,7 +986,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         const float* const g = of.g + b * of.next_g + (turned ? c0 * of.ldg : c0);
         float* const mom = of.m ? of.m + (turned ? c0 * of.ldm : c0) : nullptr;
         constexpr int AT_ONCE = 2;  // rows, of four values a lane each, which are fetched together
-        u32 least = 0xffffffffu, across[4] = {0, 0, 0, 0};
+        u32 least = 0xffffffffu, across[4] = {0, 0, 0, 0}, values[4] = {0, 0, 0, 0};
 #pragma unroll 1
         for (int i0 = warp; i0 < slow; i0 += AT_ONCE * (SMALL_THREADS / 32)) {
             float u[AT_ONCE][4], mm[AT_ONCE][4];
@@ -994,7 +1001,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
                 }
 #pragma unroll
             for (int h = 0; h < AT_ONCE; ++h) {
-                u32 most = 0;
+                u32 most = 0, found = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = i0 + h * (SMALL_THREADS / 32), j = lane + 32 * e;
@@ -1006,23 +1013,25 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
                     }
                     at_sum(turned ? j : i, turned ? i : j) = u[h][e];
                     s += (double)u[h][e] * u[h][e];
-                    most = max(most, magnitude(u[h][e])), across[e] = max(across[e], magnitude(u[h][e]));
+                    const u32 size = magnitude(u[h][e]), is = size != 0;
+                    most = max(most, size), across[e] = max(across[e], size);
+                    found += is, values[e] += is;
                 }
                 most = __reduce_max_sync(0xffffffffu, most);
-                if (most) least = min(least, most);
+                if (__reduce_add_sync(0xffffffffu, found) >= FEWEST) least = min(least, most);
             }
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (lane == 0) s_part[warp] = s, atomicMin(&s_least, least);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) atomicMax(&s_across[lane + 32 * e], across[e]);
+        for (int e = 0; e < 4; ++e) atomicMax(&s_across[lane + 32 * e], across[e]), atomicAdd(&s_values[lane + 32 * e], values[e]);
         __syncthreads();
         if (warp == 0) {
             least = s_least;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (const u32 most = s_across[lane + 32 * e]) least = min(least, most);
+                if (s_values[lane + 32 * e] >= FEWEST) least = min(least, s_across[lane + 32 * e]);
             least = __reduce_min_sync(0xffffffffu, least);
         }
         if (threadIdx.x < blocks) {

@@ -4,7 +4,7 @@
 does; ``orthogonal_step`` is the whole update of a list of weights, momentum included, and ``OrthogonalSGD`` the optimiser
 around it.  The products run on the tensor cores, with operands held to 22 bits and 2^-37 of the matrix' norm, which leaves the
 result within 1e-6 or so of itself, about as near as fp32 products.  An update with rows or columns so far below its others that
-they would lose more than 2e-4 of themselves (a stretch without a value of 2^-24 of the norm) goes by fp32 products without
+they would lose more than 2e-4 of themselves (a stretch with four or more that are not 0, and none of 2^-24 of the norm) goes by fp32 products without
 tensor cores, at a tenth of the speed, and keeps all their digits.  The reference has no training loop of its own
 (benchmark/parallel/benchmark_gcn_cpu.py:92-103 stops at the gradients).
 """

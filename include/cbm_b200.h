@@ -418,7 +418,7 @@ int cbm_b200_group_norm_grad(const void* x, int64_t ldx, const void* gy, int64_t
  *                            w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalised(U).
  *                            `of` is [host] and read before the call returns.
  * Operands of the products are held to 22 bits and 2^-37 of a matrix' norm; a matrix with a stretch of a row or column below
- * 2^-24 of its norm (but not 0) goes by fp32 products without tensor cores, about ten times as long.
+ * 2^-24 of its norm (of four values or more that are not 0) goes by fp32 products without tensor cores, about ten times as long.
  * Workspaces [dev] of the sizes given by the two functions; calls that may overlap must not share one. */
 #define CBM_B200_MAX_STEPS 64
 typedef struct {
