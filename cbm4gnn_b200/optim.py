@@ -102,6 +102,8 @@ def orthogonal_step(weights, grads, momenta, lr: float, momentum: float = 0.95, 
     written = [t.data_ptr() for t in weights + momenta if t.numel() and t.device.type != "meta"]
     if len(set(written)) < len(written):
         raise RuntimeError("orthogonal step: a weight or a momentum is there twice")
+    if not set(written).isdisjoint(g.data_ptr() for g in grads if g.numel() and g.device.type != "meta"):
+        raise RuntimeError("orthogonal step: a gradient is a weight or a momentum, too")
     with torch.no_grad():
         if dev.type != "cuda":
             for w, g, m in zip(weights, grads, momenta):
